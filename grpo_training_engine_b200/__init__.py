@@ -23,13 +23,20 @@ from . import _lib
 from .kv_pool import KVPagePool, PoolExhausted
 from .ops import (
     DecodePlan,
+    PolicyLoss,
+    add_rmsnorm_fp8,
     decode_kernel_kind,
     decode_workspace_bytes,
     gather_kv,
+    linear_fp8,
     paged_attention_decode,
     paged_kv_append,
     paged_kv_append_prompt,
     plan_decode,
+    policy_loss,
+    quantize_fp8,
+    quantize_fp8_weight,
+    token_logprobs,
 )
 from .paged_kv import paged_kv_decode as _paged_kv_decode_low_level
 from .paged_kv import paged_kv_decode_model
@@ -137,6 +144,13 @@ __all__ = [
     "decode_kernel_kind",
     "decode_workspace_bytes",
     "DecodePlan",
+    "add_rmsnorm_fp8",
+    "quantize_fp8",
+    "quantize_fp8_weight",
+    "linear_fp8",
+    "token_logprobs",
+    "policy_loss",
+    "PolicyLoss",
     "KVPagePool",
     "PoolExhausted",
 ]

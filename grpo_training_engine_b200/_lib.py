@@ -34,6 +34,11 @@ ERR_TENSOR_MAP = -6
 DEV_CTX_OUT_OF_RANGE = 1
 DEV_PAGE_OUT_OF_RANGE = 2
 DEV_WAIT_TIMEOUT = 4
+DEV_TOKEN_OUT_OF_RANGE = 8  # PKV_DEV_TOKEN_OUT_OF_RANGE
+
+REDUCE_TOKEN = 0  # PKV_REDUCE_TOKEN
+REDUCE_SEQUENCE = 1  # PKV_REDUCE_SEQUENCE
+REDUCE_SUM = 2  # PKV_REDUCE_SUM
 
 DECODE_FORCE_GENERIC = 1
 DECODE_EXACT_P = 2
@@ -46,6 +51,7 @@ LINEAR_WEIGHTS_STATIC = 0x100  # PKV_LINEAR_WEIGHTS_STATIC (flag OR'd into act)
 NOALLOC_SCRATCH_BYTES = 32 << 20  # PKV_NOALLOC_SCRATCH_BYTES in include/pkv.h
 
 _i32 = C.c_int32
+_i64 = C.c_int64
 _i64p = C.POINTER(C.c_int64)
 _vp = C.c_void_p
 _sz = C.c_size_t
@@ -105,6 +111,20 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pkv_decode_kernel_kind": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i64p, _i32, _i32, _i32]),
     "pkv_linear": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, C.c_int64, C.c_int64, C.c_int64, _i32,
                              _i32, _vp, _vp]),
+    "pkv_add_rmsnorm_fp8": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i64, _i64, _i64, _i64, _i64,
+                                      C.c_float, _i32, _vp]),
+    "pkv_quantize_fp8": (C.c_int, [_vp, _vp, _vp, _i64, _i32, _i32, _i64, _i64, _i64, _i32, _vp]),
+    "pkv_linear_fp8": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64,
+                                 _i32, _vp, _vp]),
+    "pkv_token_logprobs": (C.c_int, [_vp, _i32, _vp, _i64, _i32, _i32, _i64, _i64, C.c_float, _vp, _vp, _vp, _vp,
+                                     _vp]),
+    "pkv_token_logprobs_grad": (C.c_int, [_vp, _i32, _vp, _i64, _i32, _i32, _i64, _i64, C.c_float, _vp, _vp, _vp,
+                                          _vp, _vp, _vp]),
+    "pkv_policy_loss_workspace_size": (_sz, [_i32, _i32]),
+    "pkv_policy_loss": (C.c_int, [_vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i64, _i64,
+                                  C.c_float, C.c_float, C.c_float, C.c_float, _i32, _vp, _vp, _vp, _vp, _sz, _vp,
+                                  _vp]),
+    "pkv_scale_grad": (C.c_int, [_vp, _i64, _i32, _vp, _vp]),
 }
 
 

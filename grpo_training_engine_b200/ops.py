@@ -19,7 +19,7 @@ import contextlib
 import functools
 import math
 from dataclasses import dataclass
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -711,6 +711,367 @@ def sample_top_p(
                                  _stream(dev)),
         )
     return out
+
+
+# ---------------------------------------------------------------------------
+# 8-bit activations and weights
+# ---------------------------------------------------------------------------
+FP8_GROUP = 128  # values that share a scale
+
+
+def _fp8_rows(rows: int, cols: int, dev: torch.device) -> torch.Tensor:
+    """An e4m3 [rows, cols] tensor whose rows begin on 16-byte boundaries, as linear_fp8 reads them."""
+    wide = (cols + 15) // 16 * 16
+    q = torch.empty((rows, wide), dtype=torch.float8_e4m3fn, device=dev)
+    return q if wide == cols else q[:, :cols]
+
+
+def _groups(n: int) -> int:
+    return (n + FP8_GROUP - 1) // FP8_GROUP
+
+
+def add_rmsnorm_fp8(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    eps: float,
+    residual: Optional[torch.Tensor] = None,
+) -> tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """RMSNorm of x [rows, hidden] (after adding residual, if given) as 8-bit values, in one launch.
+
+    Returns (q, scales, x + residual or None): q float8_e4m3fn [rows, hidden]
+    and scales fp32 [rows, ceil(hidden / 128)], the norm being q times the
+    scale of its group of 128; the two are linear_fp8's x and x_scale. The norm
+    is fp32 from the unrounded sum up to q (add_rmsnorm rounds the sum and the
+    norm to x's dtype on the way); the returned sum is rounded to x's dtype.
+    Any hidden size and row strides (C ABI pkv_add_rmsnorm_fp8).
+    """
+    if x.ndim != 2 or x.stride(1) != 1:
+        raise ValueError("x must be [rows, hidden] with contiguous rows.")
+    rows, hidden = x.shape
+    if hidden == 0:
+        raise ValueError("x must have at least one column.")
+    if weight.shape != (hidden,) or weight.dtype != x.dtype or not weight.is_contiguous():
+        raise ValueError("weight must be a contiguous [hidden] tensor of x's dtype.")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.stride(1) != 1):
+        raise ValueError("residual must match x.")
+    code = _dtype_code(x, "x")
+    dev = _require_cuda(x, weight, residual)
+    q = _fp8_rows(rows, hidden, dev)
+    scales = torch.empty((rows, _groups(hidden)), dtype=torch.float32, device=dev)
+    total = torch.empty((rows, hidden), dtype=x.dtype, device=dev) if residual is not None else None
+    with _device_ctx(dev):
+        _lib.check(
+            "pkv_add_rmsnorm_fp8",
+            _lib.load().pkv_add_rmsnorm_fp8(
+                x.data_ptr(), _lib.ptr(residual), weight.data_ptr(), _lib.ptr(total), q.data_ptr(),
+                scales.data_ptr(), rows, hidden, x.stride(0), residual.stride(0) if residual is not None else 0,
+                hidden, q.stride(0), scales.stride(0), eps, code, _stream(dev)),
+        )
+    return q, scales, total
+
+
+def _quantize_fp8(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    if x.ndim != 2 or x.shape[1] == 0 or x.stride(1) != 1:
+        raise ValueError("x must be [rows, cols] with contiguous rows and at least one column.")
+    code = _dtype_code(x, "x")
+    dev = _require_cuda(x)
+    rows, cols = x.shape
+    q = _fp8_rows(rows, cols, dev)
+    scales = torch.empty(((rows + block_rows - 1) // block_rows, _groups(cols)), dtype=torch.float32, device=dev)
+    with _device_ctx(dev):
+        _lib.check(
+            "pkv_quantize_fp8",
+            _lib.load().pkv_quantize_fp8(x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, cols, block_rows,
+                                         x.stride(0), q.stride(0), scales.stride(0), code, _stream(dev)),
+        )
+    return q, scales
+
+
+def quantize_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """x [rows, cols] as (q float8_e4m3fn, scales fp32 [rows, ceil(cols / 128)]), a scale for each 128
+    values of a row: activations for linear_fp8 that no norm wrote."""
+    return _quantize_fp8(x, 1)
+
+
+def quantize_fp8_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """weight [n, k] as (q float8_e4m3fn, scales fp32 [ceil(n / 128), ceil(k / 128)]), a scale for each
+    128 x 128 block: what linear_fp8 takes. Done once when a model is loaded."""
+    return _quantize_fp8(weight, FP8_GROUP)
+
+
+def linear_fp8(
+    x: torch.Tensor,
+    x_scale: torch.Tensor,
+    weight: torch.Tensor,
+    weight_scale: torch.Tensor,
+    bias: Optional[torch.Tensor] = None,
+    *,
+    out: Optional[torch.Tensor] = None,
+    out_dtype: torch.dtype = torch.bfloat16,
+    status: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``x @ weight.T (+ bias)`` of 8-bit x [rows, K] and weight [N, K] with a scale for each 128 values of
+    a row of x and each 128 x 128 block of weight (add_rmsnorm_fp8, quantize_fp8, quantize_fp8_weight).
+
+    Any rows, N and K; fp32 accumulation, one rounding to out_dtype (bf16 or
+    fp16, also the bias's). x and weight need rows on 16-byte boundaries, as the
+    functions named lay them out (C ABI pkv_linear_fp8).
+    """
+    fp8 = torch.float8_e4m3fn
+    if x.ndim != 2 or weight.ndim != 2 or x.dtype != fp8 or weight.dtype != fp8 or x.shape[1] != weight.shape[1] \
+            or x.shape[1] == 0 or weight.shape[0] == 0:
+        raise ValueError("x [rows, K] and weight [N, K] must be float8_e4m3fn matrices of one K >= 1.")
+    rows, k = x.shape
+    n = weight.shape[0]
+    kb = _groups(k)
+    if x_scale.shape != (rows, kb) or weight_scale.shape != (_groups(n), kb) or x_scale.dtype != torch.float32 \
+            or weight_scale.dtype != torch.float32 or x_scale.stride(1) != 1 or weight_scale.stride(1) != 1:
+        raise ValueError(f"x_scale must be fp32 [rows, ceil(K / 128)] = {(rows, kb)} and weight_scale fp32 "
+                         f"[ceil(N / 128), ceil(K / 128)] = {(_groups(n), kb)}, with contiguous rows.")
+    if out is not None:
+        out_dtype = out.dtype
+    if out_dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"out_dtype must be bfloat16 or float16, got {out_dtype}.")
+    if bias is not None and (bias.shape != (n,) or bias.dtype != out_dtype or bias.stride(0) != 1):
+        raise ValueError("bias must be a contiguous [N] tensor of out_dtype.")
+    dev = _require_cuda(x, x_scale, weight, weight_scale, bias, out, status)
+    # (a single row has no stride to keep)
+    x_stride = x.stride(0) if rows > 1 else (k + 15) // 16 * 16
+    w_stride = weight.stride(0) if n > 1 else (k + 15) // 16 * 16
+    if x.stride(1) != 1 or weight.stride(1) != 1 or x_stride % 16 or w_stride % 16 or x_stride < k or w_stride < k \
+            or x.data_ptr() % 16 or weight.data_ptr() % 16:
+        raise ValueError("x and weight need contiguous rows that begin on 16-byte boundaries.")
+    if out is None:
+        out = torch.empty((rows, n), dtype=out_dtype, device=dev)
+    elif out.shape != (rows, n) or out.stride(1) != 1 or (rows > 1 and out.stride(0) < n):
+        raise ValueError(f"out must be a [rows, {n}] tensor with contiguous rows that do not overlap.")
+    with _device_ctx(dev):
+        _lib.check(
+            "pkv_linear_fp8",
+            _lib.load().pkv_linear_fp8(
+                x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(), _lib.ptr(bias),
+                out.data_ptr(), rows, n, k, x_stride, x_scale.stride(0) if rows > 1 else kb, w_stride,
+                weight_scale.stride(0) if n > FP8_GROUP else kb, out.stride(0) if rows > 1 else n,
+                _DTYPES[out_dtype], _status_ptr(status), _stream(dev)),
+        )
+    return out
+
+
+# ---------------------------------------------------------------------------
+# from logits to the policy update
+# ---------------------------------------------------------------------------
+def _logit_rows(logits: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
+    """(logits, rows, inner, outer stride, row stride) of [rows, vocab] or [batch, length, vocab] logits
+    whose vocabulary is contiguous (copied only where it is not)."""
+    if logits.stride(-1) != 1 and logits.shape[-1] > 1:
+        logits = logits.contiguous()
+    if logits.ndim == 2:
+        return logits, logits.shape[0], max(1, logits.shape[0]), 0, logits.stride(0)
+    return logits, logits.shape[0] * logits.shape[1], max(1, logits.shape[1]), logits.stride(0), logits.stride(1)
+
+
+def _check_logits(logits: torch.Tensor, tokens: torch.Tensor, temperature: float, ndims: tuple) -> None:
+    if logits.ndim not in ndims or logits.shape[-1] == 0:
+        want = " or ".join({2: "[rows, vocab]", 3: "[batch, length, vocab]"}[d] for d in ndims)
+        raise ValueError(f"logits must be {want}, got {tuple(logits.shape)}.")
+    if tokens.shape != logits.shape[:-1] or tokens.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"tokens must be int64 or int32 {tuple(logits.shape[:-1])}, got {tokens.dtype} "
+                         f"{tuple(tokens.shape)}.")
+    if not temperature > 0.0:
+        raise ValueError("temperature must be > 0.")
+
+
+def _logprobs_forward(logits, tokens, temperature, entropy, want_stats, status):
+    logits, rows, inner, outer_stride, row_stride = _logit_rows(logits)
+    dev = logits.device
+    logp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    ent = torch.empty_like(logp) if entropy else None
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None
+    with _device_ctx(dev):
+        _lib.check(
+            "pkv_token_logprobs",
+            _lib.load().pkv_token_logprobs(
+                logits.data_ptr(), _DTYPES[logits.dtype], tokens.data_ptr(), rows, logits.shape[-1], inner,
+                outer_stride, row_stride, temperature, logp.data_ptr(), _lib.ptr(ent), _lib.ptr(stats),
+                _status_ptr(status), _stream(dev)),
+        )
+    return logp, ent, stats
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, temperature, entropy, status):
+        logp, ent, stats = _logprobs_forward(logits, tokens, temperature, entropy, True, status)
+        ctx.save_for_backward(logits, tokens, stats, ent)
+        ctx.temperature = temperature
+        ctx.set_materialize_grads(False)
+        return (logp, ent) if entropy else logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_logp, d_ent=None):
+        logits, tokens, stats, ent = ctx.saved_tensors
+        if d_logp is None and d_ent is None:
+            return None, None, None, None, None
+        src, rows, inner, outer_stride, row_stride = _logit_rows(logits)
+        dev = src.device
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        d_logp, d_ent = (None if d is None else d.contiguous() for d in (d_logp, d_ent))
+        with _device_ctx(dev):
+            _lib.check(
+                "pkv_token_logprobs_grad",
+                _lib.load().pkv_token_logprobs_grad(
+                    src.data_ptr(), _DTYPES[src.dtype], tokens.data_ptr(), rows, src.shape[-1], inner, outer_stride,
+                    row_stride, ctx.temperature, stats.data_ptr(), _lib.ptr(ent), _lib.ptr(d_logp), _lib.ptr(d_ent),
+                    grad.data_ptr(), _stream(dev)),
+            )
+        return grad, None, None, None, None
+
+
+def token_logprobs(
+    logits: torch.Tensor,
+    tokens: torch.Tensor,
+    *,
+    temperature: float = 1.0,
+    entropy: bool = False,
+    status: Optional[torch.Tensor] = None,
+):
+    """Log-probability of each token under softmax(logits / temperature): fp32, tokens' shape.
+
+    logits are [rows, vocab] or [batch, length, vocab] (a ``logits[:, :-1]`` view
+    is read in place), tokens their leading shape. entropy=True returns
+    (logprobs, entropies). Differentiable in the logits through both outputs.
+    The logits are read once (and once more, with one write, for the gradient);
+    the softmax itself is never stored. A token outside [0, vocab) gives NaN and
+    sets PKV_DEV_TOKEN_OUT_OF_RANGE in status (C ABI pkv_token_logprobs).
+    """
+    _check_logits(logits, tokens, temperature, (2, 3))
+    _dtype_code(logits, "logits")
+    _require_cuda(logits, tokens, status)
+    tokens = tokens.to(torch.int64).contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _TokenLogprobs.apply(logits, tokens, float(temperature), bool(entropy), status)
+    logp, ent, _ = _logprobs_forward(logits, tokens, float(temperature), entropy, False, status)
+    return (logp, ent) if entropy else logp
+
+
+class PolicyLoss(NamedTuple):
+    """What policy_loss returns; only ``loss`` carries a gradient."""
+
+    loss: torch.Tensor           # scalar
+    logprobs: torch.Tensor       # [batch, length], 0 where the mask is 0
+    kl: torch.Tensor             # scalar: mean KL estimate over the unmasked tokens (0 without ref_logprobs)
+    clip_fraction: torch.Tensor  # scalar: share of the unmasked tokens whose ratio the clip decides
+
+
+_REDUCTIONS = {"token": _lib.REDUCE_TOKEN, "sequence": _lib.REDUCE_SEQUENCE, "sum": _lib.REDUCE_SUM}
+
+
+def _policy_forward(logits, tokens, old, ref, adv, mask, kl_coef, clip_low, clip_high, temperature, reduction,
+                    status, want_grad):
+    src, rows, _, batch_stride, row_stride = _logit_rows(logits)
+    batch, length, vocab = logits.shape
+    dev = logits.device
+    lib = _lib.load()
+    out = torch.empty(3, dtype=torch.float32, device=dev)
+    logp = torch.empty((batch, length), dtype=torch.float32, device=dev)
+    ws = torch.empty(lib.pkv_policy_loss_workspace_size(batch, length), dtype=torch.uint8, device=dev)
+    grad = torch.empty((batch, length, vocab), dtype=logits.dtype, device=dev) if want_grad else None
+    with _device_ctx(dev):
+        _lib.check(
+            "pkv_policy_loss",
+            lib.pkv_policy_loss(
+                src.data_ptr(), _DTYPES[src.dtype], tokens.data_ptr(), old.data_ptr(), _lib.ptr(ref), adv.data_ptr(),
+                adv.stride(0), adv.stride(1) if adv.ndim == 2 else 0, _lib.ptr(mask), batch, length, vocab,
+                batch_stride, row_stride, temperature, clip_low, clip_high, kl_coef, reduction, out.data_ptr(),
+                logp.data_ptr(), _lib.ptr(grad), ws.data_ptr(), ws.numel(), _status_ptr(status), _stream(dev)),
+        )
+    return out[0], logp, out[1], out[2], grad
+
+
+class _PolicyLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, *args):
+        loss, logp, kl, clipped, ctx.d_logits = _policy_forward(logits, *args, True)
+        ctx.mark_non_differentiable(logp, kl, clipped)
+        return loss, logp, kl, clipped
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_loss, *unused):
+        grad, ctx.d_logits = ctx.d_logits, None
+        if grad is None:
+            raise RuntimeError("policy_loss: its gradient was computed with the loss and has been handed out; call "
+                               "policy_loss again for another backward pass.")
+        dev = grad.device
+        with _device_ctx(dev):
+            _lib.check("pkv_scale_grad", _lib.load().pkv_scale_grad(grad.data_ptr(), grad.numel(),
+                                                                    _DTYPES[grad.dtype], d_loss.data_ptr(),
+                                                                    _stream(dev)))
+        return (grad,) + (None,) * 11
+
+
+def policy_loss(
+    logits: torch.Tensor,
+    tokens: torch.Tensor,
+    old_logprobs: torch.Tensor,
+    advantages: torch.Tensor,
+    mask: Optional[torch.Tensor] = None,
+    *,
+    ref_logprobs: Optional[torch.Tensor] = None,
+    kl_coef: float = 0.0,
+    clip_low: float = 0.2,
+    clip_high: float = 0.2,
+    temperature: float = 1.0,
+    reduction: str = "token",
+    status: Optional[torch.Tensor] = None,
+) -> PolicyLoss:
+    """Clipped policy loss with a KL term on the logits [batch, length, vocab] of the trained policy.
+
+    Per token with lp its log-probability under softmax(logits / temperature),
+    r = exp(lp - old_logprobs) and A its advantage ([batch] or [batch, length]):
+
+        -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+            + kl_coef (exp(ref - lp) - (ref - lp) - 1)
+
+    the KL term with ref_logprobs only. mask [batch, length] (bool or integer)
+    leaves tokens out: their logits are not read, whatever they hold, and get a
+    zero gradient. reduction: "token" (mean over the unmasked tokens),
+    "sequence" (mean over the batch of each sequence's mean, 0 for one without
+    tokens) or "sum".
+
+    Where the logits require grad, the same launch that computes the loss
+    writes their gradient (read once, written once); backward hands it out,
+    scaled by the upstream gradient if that is not 1, so it can run once per
+    call. The other tensors are constants (C ABI pkv_policy_loss).
+    """
+    _check_logits(logits, tokens, temperature, (3,))
+    _dtype_code(logits, "logits")
+    shape = tokens.shape
+    for name, t in (("old_logprobs", old_logprobs), ("ref_logprobs", ref_logprobs), ("mask", mask)):
+        if t is not None and t.shape != shape:
+            raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}.")
+    if advantages.shape not in (shape, shape[:1]):
+        raise ValueError(f"advantages must be {tuple(shape[:1])} or {tuple(shape)}, got {tuple(advantages.shape)}.")
+    if mask is not None and mask.is_floating_point():
+        raise ValueError("mask must be bool or integer.")
+    if not (clip_low >= 0.0 and clip_high >= 0.0):
+        raise ValueError("clip_low and clip_high must be >= 0.")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}.")
+    _require_cuda(logits, tokens, old_logprobs, advantages, mask, ref_logprobs, status)
+    if mask is not None:
+        mask = (mask if mask.dtype in (torch.bool, torch.uint8) else mask != 0).contiguous()
+    args = (
+        tokens.to(torch.int64).contiguous(),
+        old_logprobs.detach().to(torch.float32).contiguous(),
+        None if ref_logprobs is None else ref_logprobs.detach().to(torch.float32).contiguous(),
+        advantages.detach().to(torch.float32),
+        mask, float(kl_coef), float(clip_low), float(clip_high), float(temperature), _REDUCTIONS[reduction], status,
+    )
+    if logits.requires_grad and torch.is_grad_enabled():
+        return PolicyLoss(*_PolicyLossFn.apply(logits, *args))
+    return PolicyLoss(*_policy_forward(logits, *args, False)[:4])
 
 
 def decode_kernel_kind(q: torch.Tensor, k_cache: torch.Tensor, force_generic: bool = False) -> str:

@@ -37,6 +37,8 @@
 extern "C" {
 #endif
 
+/* Counts changes to entry points that exist; ones that are added (a library
+ * without them fails to resolve their names) do not raise it. */
 #define PKV_ABI_VERSION 10 /* 2: pkv_append_decode_run, 3: pkv_sample_top_p, 4: rmsnorm, rope, 5: silu_mul,
                               6: pkv_sample_top_p flags, 7: pkv_rope_qk output strides,
                               8: pkv_rope_append_decode_run, 9: pkv_linear,
@@ -66,7 +68,8 @@ enum {
 enum {
     PKV_DEV_CTX_OUT_OF_RANGE = 1,  /* context_lens[b] < 0 or > max_blocks*block_size */
     PKV_DEV_PAGE_OUT_OF_RANGE = 2, /* block_tables entry outside [0, num_blocks)      */
-    PKV_DEV_WAIT_TIMEOUT = 4       /* a bounded device-side wait gave up              */
+    PKV_DEV_WAIT_TIMEOUT = 4,      /* a bounded device-side wait gave up              */
+    PKV_DEV_TOKEN_OUT_OF_RANGE = 8 /* a token id outside [0, vocab)                   */
 };
 
 /* Decode flags. */
@@ -426,6 +429,109 @@ int pkv_decode_kernel_kind(const void *k_cache, int32_t num_q_heads,
                            int32_t num_kv_heads, int32_t head_dim,
                            int32_t block_size, const int64_t *cache_strides,
                            int32_t q_dtype, int32_t kv_dtype, int32_t flags);
+
+/* ------------------------------------------------------------------------
+ * 8-bit activations and weights: e4m3 values with a scale for each 128.
+ *
+ * pkv_add_rmsnorm_fp8: per row, s = x + residual (s = x when residual is NULL),
+ * y = weight * s / sqrt(mean(s^2) + eps), and for each 128 values of y
+ *   scale = max(max |y|, 2^-100) / 448,  q = e4m3(y / scale),
+ * so that y ~ q * scale. All of it is fp32 from the unrounded sum; sum_out
+ * (required with a residual, refused without) gets s rounded to dtype. Rows
+ * may have any length >= 1 and any stride (scale rows hold ceil(hidden / 128)
+ * values, the last group the rest of the row); sum_out and q_out may not
+ * overlap the inputs, except that sum_out may be x or residual themselves.
+ *
+ * pkv_quantize_fp8: the same scales and values for x [rows, cols], one per
+ * block_rows x 128 block; block_rows is 1 (activations) or 128 (weights).
+ * scales is [ceil(rows / block_rows), ceil(cols / 128)] with row stride
+ * scale_stride.
+ */
+int pkv_add_rmsnorm_fp8(const void *x, const void *residual, const void *weight, void *sum_out,
+                        void *q_out, float *scales, int32_t rows, int32_t hidden, int64_t x_stride,
+                        int64_t residual_stride, int64_t sum_stride, int64_t q_stride,
+                        int64_t scale_stride, float eps, int32_t dtype, void *stream);
+
+int pkv_quantize_fp8(const void *x, void *q_out, float *scales, int64_t rows, int32_t cols,
+                     int32_t block_rows, int64_t x_stride, int64_t q_stride, int64_t scale_stride,
+                     int32_t dtype, void *stream);
+
+/*
+ * pkv_linear_fp8: out[r, j] = sum_b x_scale[r, b] w_scale[j / 128, b]
+ * (sum_{k in 128 b ..} x[r, k] w[j, k]) + bias[j], for e4m3 x [rows, k] and w
+ * [n, k] with the scales above, on the tcgen05 tensor cores. fp32 accumulation
+ * within and over the blocks; out is bf16 or fp16 (out_dtype, also bias's),
+ * rounded once. Any rows, n, k >= 1 (rows 0: nothing). x and w need 16-byte
+ * aligned bases and row strides that are multiples of 16; the last block of k
+ * is read as far as k. Results do not depend on timing. No workspace.
+ */
+int pkv_linear_fp8(const void *x, const float *x_scale, const void *w, const float *w_scale,
+                   const void *bias, void *out, int32_t rows, int32_t n, int32_t k, int64_t x_stride,
+                   int64_t x_scale_stride, int64_t w_stride, int64_t w_scale_stride,
+                   int64_t out_stride, int32_t out_dtype, int32_t *status, void *stream);
+
+/* ------------------------------------------------------------------------
+ * From logits to the policy update. Row r of the logits [rows, vocab] begins at
+ * (r / inner) * outer_stride + (r % inner) * row_stride elements (a [batch,
+ * length, vocab] view needs no copy); vocab is contiguous. z = logits /
+ * temperature throughout. A token id outside [0, vocab) sets
+ * PKV_DEV_TOKEN_OUT_OF_RANGE and gives NaN; nothing is read for it.
+ *
+ * pkv_token_logprobs: logprobs[r] = log_softmax(z[r])[tokens[r]]; entropy[r]
+ * (if not NULL) the entropy of softmax(z[r]); stats (if not NULL) two floats
+ * per row, 8-byte aligned, for the gradient.
+ *
+ * pkv_token_logprobs_grad: the gradient of sum_r d_logprobs[r] logprobs[r] +
+ * d_entropy[r] entropy[r] for the logits, written to d_logits [rows, vocab]
+ * (contiguous, the logits' dtype) from the stats and entropies of the forward
+ * call. d_logprobs or d_entropy may be NULL (zero).
+ *
+ * pkv_policy_loss: for each token of [batch, length] with mask != 0 (NULL: all),
+ *   lp = log_softmax(z)[token], r = exp(lp - old),
+ *   l = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *       + kl_coef (exp(ref - lp) - (ref - lp) - 1)      (ref_logprobs given)
+ * out[0] = sum of w l with w = 1 / (number of such tokens) (PKV_REDUCE_TOKEN),
+ * 1 / (batch * number of such tokens of its sequence) (PKV_REDUCE_SEQUENCE) or
+ * 1 (PKV_REDUCE_SUM); out[1] and out[2] the mean over those tokens of the KL
+ * estimate and of whether the clip decides. logprobs [batch, length] gets lp (0
+ * where the mask is 0). d_logits (NULL: no gradient) gets d out[0] / d logits,
+ * contiguous [batch, length, vocab] of the logits' dtype, zero in rows whose
+ * mask is 0; their logits and tokens are not read. tokens, old_logprobs,
+ * ref_logprobs, mask are contiguous; advantages have two strides (0 to
+ * broadcast). The workspace is pkv_policy_loss_workspace_size bytes, 16-byte
+ * aligned, and may be reused once the call has run.
+ *
+ * pkv_scale_grad: grad[i] *= *upstream for i < n; returns without touching grad
+ * where *upstream is 1.
+ */
+enum {
+    PKV_REDUCE_TOKEN = 0,
+    PKV_REDUCE_SEQUENCE = 1,
+    PKV_REDUCE_SUM = 2
+};
+
+int pkv_token_logprobs(const void *logits, int32_t dtype, const int64_t *tokens, int64_t rows,
+                       int32_t vocab, int32_t inner, int64_t outer_stride, int64_t row_stride,
+                       float temperature, float *logprobs, float *entropy, float *stats,
+                       int32_t *status, void *stream);
+
+int pkv_token_logprobs_grad(const void *logits, int32_t dtype, const int64_t *tokens, int64_t rows,
+                            int32_t vocab, int32_t inner, int64_t outer_stride, int64_t row_stride,
+                            float temperature, const float *stats, const float *entropy,
+                            const float *d_logprobs, const float *d_entropy, void *d_logits,
+                            void *stream);
+
+size_t pkv_policy_loss_workspace_size(int32_t batch, int32_t length);
+
+int pkv_policy_loss(const void *logits, int32_t dtype, const int64_t *tokens, const float *old_logprobs,
+                    const float *ref_logprobs, const float *advantages, int64_t adv_stride_b,
+                    int64_t adv_stride_t, const uint8_t *mask, int32_t batch, int32_t length,
+                    int32_t vocab, int64_t batch_stride, int64_t row_stride, float temperature,
+                    float clip_low, float clip_high, float kl_coef, int32_t reduction, float *out,
+                    float *logprobs, void *d_logits, void *workspace, size_t workspace_bytes,
+                    int32_t *status, void *stream);
+
+int pkv_scale_grad(void *grad, int64_t n, int32_t dtype, const float *upstream, void *stream);
 
 #ifdef __cplusplus
 }
