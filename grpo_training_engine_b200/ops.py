@@ -74,7 +74,8 @@ def _as_i32(t: torch.Tensor) -> torch.Tensor:
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    # the handle alone: a Stream object per call takes 2 us of host time
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _check_cache_pair(k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
@@ -994,11 +995,14 @@ class _PolicyLossFn(torch.autograd.Function):
     def forward(ctx, logits, *args):
         loss, logp, kl, clipped, ctx.d_logits = _policy_forward(logits, *args, True)
         ctx.mark_non_differentiable(logp, kl, clipped)
+        ctx.set_materialize_grads(False)  # (no zeros for the outputs without a gradient)
         return loss, logp, kl, clipped
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_loss, *unused):
+        if d_loss is None:
+            return (None,) * 12
         grad, ctx.d_logits = ctx.d_logits, None
         if grad is None:
             raise RuntimeError("policy_loss: its gradient was computed with the loss and has been handed out; call "
