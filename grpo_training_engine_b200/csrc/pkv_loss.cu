@@ -31,8 +31,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;  // CTAs that share a row: a portable cluster
 constexpr int kUnroll = 4;      // 16-byte loads in flight per thread
-constexpr int64_t kHoldTarget = 40 * 1024;  // bytes of a row per CTA that leave room for five CTAs on an SM
-constexpr int64_t kHoldMost = 200 * 1024;   // of a longer share, what is kept in shared memory
+constexpr int kMaxBlocks = 148 * 8;  // blocks of a policy launch that have sums to add
 
 // Where row r of the logits begins: rows are (outer, inner) pairs.
 struct Rows {
@@ -64,9 +63,8 @@ struct Slice {
   bool first;
   __device__ __forceinline__ int at(int vec) const { return head + vec * kV; }  // first element of a vector
   __device__ __forceinline__ const uint4 *vecs() const { return reinterpret_cast<const uint4 *>(x + head); }
-  // The head or tail element that this thread has, or -1.
-  __device__ __forceinline__ int edge() const {
-    const int t = threadIdx.x;
+  // The head or tail element that thread t of those that share the slice has, or -1.
+  __device__ __forceinline__ int edge(int t) const {
     if (first && t < head) return t;
     return t >= kV && t < kV + tail ? tail0 + t - kV : -1;
   }
@@ -111,6 +109,12 @@ template <> struct Vec<float> {
     return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)),
                    max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
   }
+  static __device__ __forceinline__ uint4 max4(uint4 a, uint4 b) {
+    return make_uint4(max2(a.x, b.x), max2(a.y, b.y), max2(a.z, b.z), max2(a.w, b.w));
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+  }
   static __device__ __forceinline__ uint4 pack(const float2 (&f)[2]) {
     return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x),
                       __float_as_uint(f[1].y));
@@ -128,6 +132,9 @@ template <> struct Vec<__nv_bfloat16> {
     uint32_t r;
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
+  }
+  static __device__ __forceinline__ uint4 max4(uint4 a, uint4 b) {
+    return make_uint4(max2(a.x, b.x), max2(a.y, b.y), max2(a.z, b.z), max2(a.w, b.w));
   }
   static __device__ __forceinline__ float max(uint4 v) {
     const float2 m = pair(max2(max2(v.x, v.y), max2(v.z, v.w)));
@@ -154,6 +161,9 @@ template <> struct Vec<__half> {
     uint32_t r;
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
+  }
+  static __device__ __forceinline__ uint4 max4(uint4 a, uint4 b) {
+    return make_uint4(max2(a.x, b.x), max2(a.y, b.y), max2(a.z, b.z), max2(a.w, b.w));
   }
   static __device__ __forceinline__ float max(uint4 v) {
     const float2 m = pair(max2(max2(v.x, v.y), max2(v.z, v.w)));
@@ -201,24 +211,43 @@ __device__ __forceinline__ void add(Soft &a, float x, float c) {
   if (Entropy) a.w += weighted(e, t);
 }
 
-// A vector: its exponentials are added to each other before they are added to
-// the running sum, which keeps what is small beside a dominant entry.
-template <typename T, bool Entropy>
-__device__ __forceinline__ void add_vec(Soft &a, uint4 v, float c) {
+// N vectors: one look at the maximum, and their exponentials are added to each
+// other before they are added to the running sum, which keeps what is small
+// beside a dominant entry.
+template <typename T, bool Entropy, int N>
+__device__ __forceinline__ void add_vecs(Soft &a, const uint4 (&v)[N], float c) {
   constexpr int P = Vec<T>::kPairs;
-  const float vm = Vec<T>::max(v);
+  uint4 top = v[0];
+#pragma unroll
+  for (int n = 1; n < N; ++n) top = Vec<T>::max4(top, v[n]);
+  const float vm = Vec<T>::max(top);
   if (!(vm <= a.m)) rescale<Entropy>(a, max_nan(a.m, vm), c);
-  float2 f[P], s = make_float2(0.f, 0.f), w = s;
-  Vec<T>::unpack(v, f);
+  float2 s = make_float2(0.f, 0.f), w = s;
   const float2 nm = make_float2(-a.m, -a.m), cc = make_float2(c, c);
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const float2 t = mul2(add2(f[i], nm), cc), e = make_float2(fast_exp2(t.x), fast_exp2(t.y));
-    s = i == 0 ? e : add2(s, e);
-    if (Entropy) w = fma2(e, make_float2(fmaxf(t.x, -1e4f), fmaxf(t.y, -1e4f)), w);
+  for (int n = 0; n < N; ++n) {
+    float2 f[P];
+    Vec<T>::unpack(v[n], f);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float2 t = mul2(add2(f[i], nm), cc), e = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+      s = n + i == 0 ? e : add2(s, e);
+      if (Entropy) w = fma2(e, make_float2(fmaxf(t.x, -1e4f), fmaxf(t.y, -1e4f)), w);
+    }
   }
   a.s += s.x + s.y;
   if (Entropy) a.w += w.x + w.y;
+}
+
+__device__ __forceinline__ void mbar_expect(uint64_t *bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
+// Barrier of the block's first NT threads.
+template <int NT>
+__device__ __forceinline__ void bar_sync() {
+  __syncwarp();
+  asm volatile("barrier.sync 1, %0;" ::"n"(NT) : "memory");
 }
 
 __device__ __forceinline__ void cluster_arrive() {
@@ -231,10 +260,8 @@ struct Joint {
   Soft cta[kMaxCluster];  // written by the CTAs of the cluster
 };
 
-// Joined over the block and over the CTAs that share the row (the caller has
-// arrived at the cluster barrier once); every thread returns the same values.
 template <bool Entropy>
-__device__ __forceinline__ Soft row_join(Soft a, float c, Joint &red, int rank, int ctas) {
+__device__ __forceinline__ void warp_join(Soft &a, float c) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     Soft b;
@@ -243,6 +270,13 @@ __device__ __forceinline__ Soft row_join(Soft a, float c, Joint &red, int rank, 
     b.w = Entropy ? __shfl_xor_sync(0xffffffffu, a.w, o) : 0.f;
     join<Entropy>(a, b, c);
   }
+}
+
+// Joined over the block and over the CTAs that share the row (the caller has
+// arrived at the cluster barrier once); every thread returns the same values.
+template <bool Entropy>
+__device__ __forceinline__ Soft row_join(Soft a, float c, Joint &red, int rank, int ctas) {
+  warp_join<Entropy>(a, c);
   if ((threadIdx.x & 31) == 0) red.warp[threadIdx.x >> 5] = a;
   __syncthreads();
   a = red.warp[0];
@@ -265,48 +299,79 @@ __device__ __forceinline__ Soft row_join(Soft a, float c, Joint &red, int rank, 
   return a;
 }
 
-// This thread's part of a slice, streamed from global memory from vector `lo` on.
-template <typename T, bool Entropy>
-__device__ __forceinline__ void add_stream(Soft &a, const Slice<T> &sl, int lo, float c) {
-  const uint4 *p = sl.vecs();
-  int i = lo + (int)threadIdx.x;
-  for (; i + (kUnroll - 1) * kThreads < sl.hi; i += kUnroll * kThreads) {
+// Thread tid's part (of NT) of n vectors in global (Ldg) or shared memory.
+template <typename T, bool Entropy, int NT, bool Ldg>
+__device__ __forceinline__ void add_range(Soft &a, const uint4 *p, int n, float c, int tid) {
+  int i = tid;
+  for (; i + (kUnroll - 1) * NT < n; i += kUnroll * NT) {
     uint4 v[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) v[u] = __ldg(p + i + u * kThreads);
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) add_vec<T, Entropy>(a, v[u], c);
+    for (int u = 0; u < kUnroll; ++u) v[u] = Ldg ? __ldg(p + i + u * NT) : p[i + u * NT];
+    add_vecs<T, Entropy, kUnroll>(a, v, c);
   }
-  for (; i < sl.hi; i += kThreads) add_vec<T, Entropy>(a, __ldg(p + i), c);
+  for (; i < n; i += NT) {
+    const uint4 v[1] = {Ldg ? __ldg(p + i) : p[i]};
+    add_vecs<T, Entropy, 1>(a, v, c);
+  }
 }
 
 // ---------------------------------------------------------------------------
 // token log-probabilities
 // ---------------------------------------------------------------------------
+struct LogprobArgs {
+  const int64_t *tokens;
+  float *logp, *entropy;  // entropy: with Entropy only
+  float2 *stats;          // m and s of each row, or nullptr
+  int32_t *status;
+  int64_t rows;
+  int32_t vocab, ctas;
+  float inv_t, c;
+};
+
+// One thread per row, from the row's joined sums.
 template <typename T, bool Entropy>
-__global__ void __launch_bounds__(kThreads)
-logprob_kernel(const T *logits, Rows rows, const int64_t *tokens, int vocab, int ctas, float inv_t, float c,
-               float *logp, float *entropy, float2 *stats, int32_t *status) {
+__device__ __forceinline__ void store_logprob(const LogprobArgs &p, const T *x, int64_t r, const Soft &a) {
+  const int64_t tok = p.tokens[r];
+  const bool in = tok >= 0 && tok < p.vocab;
+  const float lns = logf(a.s);
+  if (!in) flag_status(p.status, PKV_DEV_TOKEN_OUT_OF_RANGE);
+  p.logp[r] = in ? (Elem<T>::to_f32(x[tok]) - a.m) * p.inv_t - lns : NAN;
+  if (Entropy) p.entropy[r] = lns - kLn2 * (a.w / a.s);
+  if (p.stats != nullptr) p.stats[r] = make_float2(a.m, a.s);
+}
+
+// A block, or the blocks of a cluster, per row.
+template <typename T, bool Entropy>
+__global__ void __launch_bounds__(kThreads) logprob_kernel(const T *logits, Rows rows, LogprobArgs p) {
   __shared__ Joint red;
-  if (ctas > 1) cluster_arrive();
-  const int64_t r = blockIdx.x / ctas;
-  const int rank = blockIdx.x % ctas;
+  if (p.ctas > 1) cluster_arrive();
+  const int64_t r = blockIdx.x / p.ctas;
+  const int rank = blockIdx.x % p.ctas;
   const T *x = logits + rows.offset(r);
-  const Slice<T> sl(x, vocab, rank, ctas);
+  const Slice<T> sl(x, p.vocab, rank, p.ctas);
   Soft a;
-  add_stream<T, Entropy>(a, sl, sl.lo, c);
-  const int e = sl.edge();
-  if (e >= 0) add<Entropy>(a, Elem<T>::to_f32(x[e]), c);
-  a = row_join<Entropy>(a, c, red, rank, ctas);
-  if (rank == 0 && threadIdx.x == 0) {
-    const int64_t tok = tokens[r];
-    const bool in = tok >= 0 && tok < vocab;
-    const float lns = logf(a.s);
-    if (!in) flag_status(status, PKV_DEV_TOKEN_OUT_OF_RANGE);
-    logp[r] = in ? (Elem<T>::to_f32(x[tok]) - a.m) * inv_t - lns : NAN;
-    if (Entropy) entropy[r] = lns - kLn2 * (a.w / a.s);
-    if (stats != nullptr) stats[r] = make_float2(a.m, a.s);
-  }
+  add_range<T, Entropy, kThreads, true>(a, sl.vecs() + sl.lo, sl.hi - sl.lo, p.c, threadIdx.x);
+  const int e = sl.edge(threadIdx.x);
+  if (e >= 0) add<Entropy>(a, Elem<T>::to_f32(x[e]), p.c);
+  a = row_join<Entropy>(a, p.c, red, rank, p.ctas);
+  if (rank == 0 && threadIdx.x == 0) store_logprob<T, Entropy>(p, x, r, a);
+}
+
+// A warp per row, for rows that would leave most of a block idle.
+template <typename T, bool Entropy>
+__global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const T *logits, Rows rows, LogprobArgs p) {
+  const int64_t r = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
+  const int lane = threadIdx.x & 31;
+  if (r >= p.rows) return;
+  const T *x = logits + rows.offset(r);
+  const Slice<T> sl(x, p.vocab, 0, 1);
+  Soft a;
+  add_range<T, Entropy, 32, true>(a, sl.vecs(), sl.hi, p.c, lane);
+  const int e = sl.edge(lane);
+  if (e >= 0) add<Entropy>(a, Elem<T>::to_f32(x[e]), p.c);
+  __syncwarp();
+  warp_join<Entropy>(a, p.c);
+  if (lane == 0) store_logprob<T, Entropy>(p, x, r, a);
 }
 
 // Gradient of one element from t = (x - m) c and e = 2^t: e (a + b t), and `hot` more at the token.
@@ -322,9 +387,8 @@ __device__ __forceinline__ float grad_of(const Slope &g, float x, int v) {
   return v == g.tok ? d + g.hot : d;
 }
 
-// v0: the vector's first element
 template <typename T, bool Entropy>
-__device__ __forceinline__ uint4 grad_vec(const Slope &g, uint4 v, int v0) {
+__device__ __forceinline__ uint4 grad_vec(const Slope &g, uint4 v) {
   constexpr int P = Vec<T>::kPairs;
   float2 f[P];
   Vec<T>::unpack(v, f);
@@ -335,58 +399,62 @@ __device__ __forceinline__ uint4 grad_vec(const Slope &g, uint4 v, int v0) {
     const float2 t = mul2(add2(f[i], nm), cc), e = make_float2(fast_exp2(t.x), fast_exp2(t.y));
     f[i] = Entropy ? mul2(e, fma2(gb, make_float2(fmaxf(t.x, -1e4f), fmaxf(t.y, -1e4f)), ga)) : mul2(e, ga);
   }
-  const int64_t k = g.tok - v0;
-  if (k >= 0 && k < 2 * P) {
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      if (k == 2 * i) f[i].x += g.hot;
-      if (k == 2 * i + 1) f[i].y += g.hot;
-    }
-  }
   return Vec<T>::pack(f);
 }
 
-// The gradient of this CTA's slice: from shared memory up to vector `held`,
-// from global memory (the second read: L2) beyond. `out` is the row's gradient;
-// where its vectors do not begin where the logits' do, elements go one by one.
-template <typename T, bool Entropy>
-__device__ __forceinline__ void grad_slice(const Slice<T> &sl, const Slope &g, T *out, const uint4 *held_v, int held) {
+// The gradient of the row's vectors [i0, i1), from `src` (i0's place, in global
+// or shared memory). Where the vectors of the gradient's row do not begin where
+// the logits' do, elements go one by one. The token's element gets its share
+// from the thread that stored its vector.
+template <typename T, bool Entropy, int NT>
+__device__ __forceinline__ void grad_range(const Slice<T> &sl, const Slope &g, T *out, const uint4 *src, int i0,
+                                           int i1, int tid) {
   if ((reinterpret_cast<uintptr_t>(out + sl.head) & 15) == 0) {
-    uint4 *o = reinterpret_cast<uint4 *>(out + sl.head);
-    for (int i = sl.lo + (int)threadIdx.x; i < held; i += kThreads)
-      __stcs(o + i, grad_vec<T, Entropy>(g, held_v[i - sl.lo], sl.at(i)));
-    int i = held + (int)threadIdx.x;
-    for (; i + (kUnroll - 1) * kThreads < sl.hi; i += kUnroll * kThreads) {
+    uint4 *o = reinterpret_cast<uint4 *>(out + sl.head) + i0;
+    const int n = i1 - i0;
+    int i = tid;
+    for (; i + (kUnroll - 1) * NT < n; i += kUnroll * NT) {
       uint4 v[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) v[u] = __ldg(sl.vecs() + i + u * kThreads);
+      for (int u = 0; u < kUnroll; ++u) v[u] = src[i + u * NT];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u)
-        __stcs(o + i + u * kThreads, grad_vec<T, Entropy>(g, v[u], sl.at(i + u * kThreads)));
+        __stcs(o + i + u * NT, grad_vec<T, Entropy>(g, v[u]));
     }
-    for (; i < sl.hi; i += kThreads) __stcs(o + i, grad_vec<T, Entropy>(g, __ldg(sl.vecs() + i), sl.at(i)));
+    for (; i < n; i += NT) __stcs(o + i, grad_vec<T, Entropy>(g, src[i]));
+    const int64_t k = g.tok - sl.at(i0);  // the token's place in the range
+    if (k >= 0 && k < (int64_t)n * Slice<T>::kV && (int)(k / Slice<T>::kV) % NT == tid)
+      out[g.tok] = from_f32<T>(grad_of<Entropy>(g, Elem<T>::to_f32(reinterpret_cast<const T *>(src)[k]), (int)g.tok));
   } else {
-    const T *h = reinterpret_cast<const T *>(held_v);
-    for (int v = sl.at(sl.lo) + (int)threadIdx.x; v < sl.at(held); v += kThreads)
-      out[v] = from_f32<T>(grad_of<Entropy>(g, Elem<T>::to_f32(h[v - sl.at(sl.lo)]), v));
-    for (int v = sl.at(held) + (int)threadIdx.x; v < sl.at(sl.hi); v += kThreads)
-      out[v] = from_f32<T>(grad_of<Entropy>(g, Elem<T>::to_f32(sl.x[v]), v));
+    const T *e = reinterpret_cast<const T *>(src);
+    const int v0 = sl.at(i0), n = (i1 - i0) * Slice<T>::kV;
+    for (int i = tid; i < n; i += NT)
+      out[v0 + i] = from_f32<T>(grad_of<Entropy>(g, Elem<T>::to_f32(e[i]), v0 + i));
   }
-  const int e = sl.edge();
-  if (e >= 0) out[e] = from_f32<T>(grad_of<Entropy>(g, Elem<T>::to_f32(sl.x[e]), e));
 }
 
 template <typename T, bool Entropy>
+__device__ __forceinline__ void grad_edge(const Slice<T> &sl, const Slope &g, T *out, int tid) {
+  const int e = sl.edge(tid);
+  if (e >= 0) out[e] = from_f32<T>(grad_of<Entropy>(g, Elem<T>::to_f32(sl.x[e]), e));
+}
+
+// NT threads per row or per share of a row (p.ctas of them).
+template <typename T, bool Entropy, int NT>
 __global__ void __launch_bounds__(kThreads)
-logprob_grad_kernel(const T *logits, Rows rows, const int64_t *tokens, int vocab, int ctas, float inv_t, float c,
-                    const float2 *stats, const float *entropy, const float *d_logp, const float *d_entropy, T *grad) {
-  const int64_t r = blockIdx.x / ctas;
-  const Slice<T> sl(logits + rows.offset(r), vocab, blockIdx.x % ctas, ctas);
-  const float2 st = stats[r];
-  const float g = d_logp != nullptr ? d_logp[r] : 0.f, h = Entropy ? d_entropy[r] : 0.f, k = inv_t / st.y;
+logprob_grad_kernel(const T *logits, Rows rows, LogprobArgs p, const float *d_logp, const float *d_entropy, T *grad) {
+  const int64_t at = (int64_t)blockIdx.x * (kThreads / NT) + threadIdx.x / NT, r = at / p.ctas;
+  const int tid = threadIdx.x % NT;
+  if (r >= p.rows) return;
+  const Slice<T> sl(logits + rows.offset(r), p.vocab, (int)(at % p.ctas), p.ctas);
+  const float2 st = p.stats[r];
+  const float g = d_logp != nullptr ? d_logp[r] : 0.f, h = Entropy ? d_entropy[r] : 0.f, k = p.inv_t / st.y;
   // -p (g + h (log p + H)) / T with log p = t ln2 - ln s
-  Slope sp{st.x, c, Entropy ? -k * (g + h * (entropy[r] - logf(st.y))) : -k * g, -h * kLn2 * k, g * inv_t, tokens[r]};
-  grad_slice<T, Entropy>(sl, sp, grad + r * (int64_t)vocab, nullptr, sl.lo);
+  const Slope sp{st.x, p.c, Entropy ? -k * (g + h * (p.entropy[r] - logf(st.y))) : -k * g, -h * kLn2 * k,
+                 g * p.inv_t, p.tokens[r]};
+  T *out = grad + r * (int64_t)p.vocab;
+  grad_range<T, Entropy, NT>(sl, sp, out, sl.vecs() + sl.lo, sl.lo, sl.hi, tid);
+  grad_edge<T, Entropy>(sl, sp, out, tid);
 }
 
 // ---------------------------------------------------------------------------
@@ -400,190 +468,450 @@ struct PolicyArgs {
   const uint8_t *mask;     // [batch, length] or nullptr
   float *out;              // loss, kl, clipped fraction
   float *logp;             // [batch, length]
-  float4 *terms;           // workspace [batch * length]: w l, kl, clipped
-  float *weight;           // workspace [batch * length]
+  double *partial;         // workspace [3 * kMaxBlocks]: each block's sums
   int32_t *order;          // workspace [batch * length]: tokens with a weight first
   int32_t *before;         // workspace [batch + 1]: such tokens before each sequence
-  int32_t *counts;         // workspace: [0] tokens with a weight, [1] rows done
+  int32_t *counts;         // workspace: [0] tokens with a weight, [1] blocks done
   int32_t *status;
   int64_t adv_b, adv_t;
-  int32_t batch, length, vocab, reduction, ctas, hold;  // hold: vectors of a slice kept in shared memory
+  int32_t batch, length, vocab, reduction;
+  int32_t ctas, hold;  // CTAs of a row (loss alone); vectors of a row kept in shared memory (gradient)
   float inv_t, c, clip_low, clip_high, kl_coef;
 };
 
 constexpr int kPrepThreads = 1024;
 
-// One block: the tokens with a weight in front, each one's weight, counters.
-// A running count over the tokens, kept at each sequence's start, gives the
-// sequences' lengths.
-__global__ void __launch_bounds__(kPrepThreads) policy_prep_kernel(PolicyArgs a) {
-  __shared__ int warp_sum[kPrepThreads / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t n = (int64_t)a.batch * a.length;
-  int mine = 0;
-  const int64_t per = (n + kPrepThreads - 1) / kPrepThreads, lo = min(n, tid * per), hi = min(n, lo + per);
-  for (int64_t i = lo; i < hi; ++i) mine += a.mask == nullptr || a.mask[i] != 0;
-  int incl = mine;
+// Non-zero bytes among mask[0, n) that this thread of the block looks at.
+__device__ __forceinline__ int count_mask(const uint8_t *mask, int64_t n) {
+  int count = 0;
+  int64_t i = threadIdx.x;
+  if ((reinterpret_cast<uintptr_t>(mask) & 15) == 0) {
+    for (; i < n / 16; i += kPrepThreads) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4 *>(mask) + i);
+      count += __popc(__vsetne4(v.x, 0)) + __popc(__vsetne4(v.y, 0)) + __popc(__vsetne4(v.z, 0)) +
+               __popc(__vsetne4(v.w, 0));
+    }
+    i = n / 16 * 16 + threadIdx.x;
+  }
+  for (; i < n; i += kPrepThreads) count += mask[i] != 0;
+  return count;
+}
+
+// Sum over the block; every thread returns it.
+__device__ __forceinline__ int block_sum(int v, int *red) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
-  }
-  if (lane == 31) warp_sum[warp] = incl;
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();
-  int total = 0, start = incl - mine;
-  for (int i = 0; i < kPrepThreads / 32; ++i) {
-    if (i < warp) start += warp_sum[i];
-    total += warp_sum[i];
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0;
+  for (int i = 0; i < kPrepThreads / 32; ++i) v += red[i];
+  return v;
+}
+
+// The tokens with a weight in front, and how many of them there are before each
+// sequence. One token per thread; each block counts what lies before and behind
+// its tokens itself (a byte per token, from L2), so one launch does.
+__global__ void __launch_bounds__(kPrepThreads) policy_prep_kernel(PolicyArgs a) {
+  __shared__ int red[kPrepThreads / 32];
+  const int64_t n = (int64_t)a.batch * a.length, base = (int64_t)blockIdx.x * kPrepThreads, i = base + threadIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool on = i < n && (a.mask == nullptr || a.mask[i] != 0);
+  const uint32_t votes = __ballot_sync(0xffffffffu, on);
+  int before = (int)base, total = (int)n;
+  if (a.mask != nullptr) {
+    before = block_sum(count_mask(a.mask, base), red);
+    total = block_sum(count_mask(a.mask, n), red);
   }
-  if (tid == 0) {
+  __syncthreads();
+  if (lane == 0) red[warp] = __popc(votes);
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) before += red[w];
+  before += __popc(votes & ((1u << lane) - 1));
+  if (i < n) {
+    a.order[on ? before : total + (int)i - before] = (int32_t)i;
+    if (i % a.length == 0) a.before[i / a.length] = before;
+  }
+  if (i == 0) {
     a.before[a.batch] = total;
     a.counts[0] = total;
     a.counts[1] = 0;
   }
-  int active = start, idle = total + (int)lo - start;
-  for (int64_t i = lo; i < hi; ++i) {
-    if (i % a.length == 0) a.before[i / a.length] = active;
-    const bool on = a.mask == nullptr || a.mask[i] != 0;
-    a.order[on ? active++ : idle++] = (int32_t)i;
-  }
-  __syncthreads();
-  for (int64_t i = tid; i < n; i += kPrepThreads) {
-    const int64_t b = i / a.length;
-    const int len = a.before[b + 1] - a.before[b];
-    a.weight[i] = a.reduction == PKV_REDUCE_TOKEN      ? 1.f / (float)max(1, total)
-                  : a.reduction == PKV_REDUCE_SEQUENCE ? 1.f / ((float)max(1, len) * (float)a.batch)
-                                                       : 1.f;
-  }
 }
 
-constexpr int kChunks = 4;  // bulk copies of a slice: the first is worked on while the last arrive
+// A token's inputs.
+struct TokenIn {
+  int64_t tok;
+  float x, old, ref, adv;  // x: the token's logit
+  int len;                 // tokens with a weight that share the token's weight's normaliser
+  bool in;
+};
 
-// One cluster per row. With a gradient the row is read once into the shared
-// memory of the cluster's CTAs by bulk copies, summed from there, and its
-// gradient written from there.
-template <typename T, bool Grad>
-__global__ void __launch_bounds__(kThreads)
-policy_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
-  extern __shared__ __align__(16) uint8_t held_raw[];
-  __shared__ Joint red;
-  __shared__ uint64_t bars[kChunks];
-  __shared__ float slope_s;
-  __shared__ int last_s;
-  if (a.ctas > 1) cluster_arrive();
-  const int64_t pos = blockIdx.x / a.ctas, r = a.order[pos];
-  const int rank = blockIdx.x % a.ctas, tid = threadIdx.x;
-  T *out = grad + r * (int64_t)a.vocab;
-  if (pos >= a.counts[0]) {
-    if (a.ctas > 1) cluster_wait();
-    if (Grad) {
-      const Slice<T> sl(out, a.vocab, rank, a.ctas);
-      uint4 *o = reinterpret_cast<uint4 *>(out + sl.head);
-      for (int i = sl.lo + tid; i < sl.hi; i += kThreads) __stcs(o + i, make_uint4(0, 0, 0, 0));
-      const int e = sl.edge();
-      if (e >= 0) out[e] = from_f32<T>(0.f);
-    }
-    if (rank == 0 && tid == 0) {
-      a.logp[r] = 0.f;
-      a.terms[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-  } else {
-    const T *x = logits + rows.offset(r);
-    const Slice<T> sl(x, a.vocab, rank, a.ctas);
-    const uint4 *hv = reinterpret_cast<const uint4 *>(held_raw);
-    const int held = Grad ? min(sl.hi, sl.lo + a.hold) : sl.lo, n_held = held - sl.lo;
-    if (Grad) {
-      if (tid == 0) {
-        for (int k = 0; k < kChunks; ++k) mbar_init(&bars[k], 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        for (int k = 0; k < kChunks; ++k) {
-          const int c0 = (int)((int64_t)n_held * k / kChunks), c1 = (int)((int64_t)n_held * (k + 1) / kChunks);
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&bars[k])),
-                       "r"((c1 - c0) * 16)
-                       : "memory");
-          if (c1 > c0)
-            asm volatile(
-                "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                    smem_u32(hv + c0)),
-                "l"(sl.vecs() + sl.lo + c0), "r"((c1 - c0) * 16), "r"(smem_u32(&bars[k]))
-                : "memory");
-        }
-      }
-      __syncthreads();
-    }
-    Soft st;
-    const int e = sl.edge();
-    if (e >= 0) add<false>(st, Elem<T>::to_f32(x[e]), a.c);
-    bool ok = true;
-    if (Grad) {
-      for (int k = 0; k < kChunks; ++k) {
-        const int c0 = (int)((int64_t)n_held * k / kChunks), c1 = (int)((int64_t)n_held * (k + 1) / kChunks);
-        ok = mbar_wait_bounded(&bars[k], 0) && ok;
-        for (int i = c0 + tid; i < c1; i += kThreads) add_vec<T, false>(st, hv[i], a.c);
-      }
-      if (!ok) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
-    }
-    add_stream<T, false>(st, sl, held, a.c);
-    st = row_join<false>(st, a.c, red, rank, a.ctas);
-    const int64_t tok = a.tokens[r];
-    if (tid == 0) {
-      const float w = a.weight[r];
-      const bool in = tok >= 0 && tok < a.vocab;
-      const float lp = in ? (Elem<T>::to_f32(x[tok]) - st.m) * a.inv_t - logf(st.s) : NAN;
-      const float adv = a.adv[(r / a.length) * a.adv_b + (r % a.length) * a.adv_t];
-      const float ratio = expf(lp - a.old_logp[r]);
-      const float free = ratio * adv, clip = fminf(fmaxf(ratio, 1.f - a.clip_low), 1.f + a.clip_high) * adv;
-      const bool clipped = clip < free;
-      float l = clipped ? -clip : -free, slope = clipped ? 0.f : -free, kl = 0.f;
-      if (a.ref_logp != nullptr) {
-        const float d = a.ref_logp[r] - lp, em = expm1f(d);
-        kl = em - d;
-        l += a.kl_coef * kl;
-        slope -= a.kl_coef * em;
-      }
-      slope_s = slope * w * a.inv_t;
-      if (rank == 0) {
-        if (!in) flag_status(a.status, PKV_DEV_TOKEN_OUT_OF_RANGE);
-        a.logp[r] = lp;
-        a.terms[r] = make_float4(w * l, kl, clipped ? 1.f : 0.f, 0.f);
-      }
-    }
-    __syncthreads();
-    if (Grad) grad_slice<T, false>(sl, Slope{st.m, a.c, -slope_s / st.s, 0.f, slope_s, tok}, out, hv, held);
+template <typename T>
+__device__ __forceinline__ TokenIn token_in(const PolicyArgs &a, const T *x, int64_t r) {
+  TokenIn t;
+  const int b = (int)r / a.length;
+  t.tok = a.tokens[r];
+  t.in = t.tok >= 0 && t.tok < a.vocab;
+  t.old = a.old_logp[r];
+  t.ref = a.ref_logp != nullptr ? a.ref_logp[r] : 0.f;
+  t.adv = a.adv[b * a.adv_b + ((int)r - b * a.length) * a.adv_t];
+  t.len = a.reduction == PKV_REDUCE_SEQUENCE ? a.before[b + 1] - a.before[b] : a.counts[0];
+  t.x = t.in ? Elem<T>::to_f32(x[t.tok]) : 0.f;
+  return t;
+}
+
+// Sums over a block's tokens: the weighted loss (its constant factor left out),
+// the KL estimate, the clipped tokens.
+struct Sums {
+  double loss = 0, kl = 0, clipped = 0;
+};
+
+// What a row's gradient needs: the maximum, the factor of the exponentials, the
+// slope at the token.
+struct RowResult {
+  float m, k, slope;
+  int64_t tok;
+};
+
+// One thread per row, from the row's joined sums: its log-probability, its
+// share of the sums, and what its gradient needs.
+__device__ __forceinline__ RowResult token_result(const PolicyArgs &a, const TokenIn &t, const Soft &st, int64_t r,
+                                                  Sums &sums) {
+  const float lp = t.in ? (t.x - st.m) * a.inv_t - logf(st.s) : NAN;
+  const float ratio = expf(lp - t.old);
+  const float free = ratio * t.adv, clip = fminf(fmaxf(ratio, 1.f - a.clip_low), 1.f + a.clip_high) * t.adv;
+  const bool clipped = clip < free;
+  float l = clipped ? -clip : -free, slope = clipped ? 0.f : -free, kl = 0.f;
+  if (a.ref_logp != nullptr) {
+    const float d = t.ref - lp, em = expm1f(d);
+    kl = em - d;
+    l += a.kl_coef * kl;
+    slope -= a.kl_coef * em;
   }
-  if (rank != 0) return;
-  // the last row's CTA adds the rows' terms in row order, in 64 bits
-  const int64_t n = (int64_t)a.batch * a.length;
+  if (!t.in) flag_status(a.status, PKV_DEV_TOKEN_OUT_OF_RANGE);
+  a.logp[r] = lp;
+  sums.loss += a.reduction == PKV_REDUCE_SEQUENCE ? (double)l / t.len : (double)l;
+  sums.kl += kl;
+  sums.clipped += clipped;
+  const float w = a.reduction == PKV_REDUCE_SUM        ? 1.f
+                  : a.reduction == PKV_REDUCE_SEQUENCE ? 1.f / ((float)t.len * (float)a.batch)
+                                                       : 1.f / (float)t.len;
+  slope *= w * a.inv_t;
+  return RowResult{st.m, -slope / st.s, slope, t.tok};
+}
+
+// Called by the NT threads of a block with its sums in thread 0: the block that
+// comes last of `blocks` adds the blocks' sums in their order. Each block's
+// tokens and their order are fixed, so the result does not depend on timing.
+template <int NT>
+__device__ __forceinline__ void finish(const PolicyArgs &a, const Sums &mine, int block, int blocks) {
+  __shared__ double sums[3][NT / 32];
+  __shared__ int last_s;
+  const int tid = threadIdx.x;
   if (tid == 0) {
+    a.partial[3 * block] = mine.loss;
+    a.partial[3 * block + 1] = mine.kl;
+    a.partial[3 * block + 2] = mine.clipped;
     __threadfence();
-    last_s = atomicAdd(&a.counts[1], 1) == (int)n - 1;
+    last_s = atomicAdd(&a.counts[1], 1) == blocks - 1;
   }
   __syncthreads();
   if (!last_s) return;
   __threadfence();
-  __shared__ double sums[3][kThreads];
-  double l = 0, kl = 0, cl = 0;
-  for (int64_t i = tid; i < n; i += kThreads) {
-    const float4 t = __ldcg(a.terms + i);
-    l += t.x;
-    kl += t.y;
-    cl += t.z;
+  double v[3] = {0, 0, 0};
+#pragma unroll 4
+  for (int i = tid; i < blocks; i += NT) {
+    v[0] += __ldcg(a.partial + 3 * i);
+    v[1] += __ldcg(a.partial + 3 * i + 1);
+    v[2] += __ldcg(a.partial + 3 * i + 2);
   }
-  sums[0][tid] = l;
-  sums[1][tid] = kl;
-  sums[2][tid] = cl;
-  for (int o = kThreads / 2; o > 0; o >>= 1) {
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[j] += __shfl_xor_sync(0xffffffffu, v[j], o);
+    if ((tid & 31) == 0) sums[j][tid >> 5] = v[j];
+  }
+  __syncthreads();
+  if (tid < 3) {
+    const double tokens = max(1, a.counts[0]);
+    double t = 0;
+    for (int i = 0; i < NT / 32; ++i) t += sums[tid][i];
+    if (tid > 0 || a.reduction == PKV_REDUCE_TOKEN) t /= tokens;
+    if (tid == 0 && a.reduction == PKV_REDUCE_SEQUENCE) t /= a.batch;
+    a.out[tid] = (float)t;
+  }
+}
+
+// The loss alone. A cluster takes every row_step-th row (one each where rows
+// are shared), streamed.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) policy_kernel(const T *logits, Rows rows, PolicyArgs a) {
+  __shared__ Joint red;
+  if (a.ctas > 1) cluster_arrive();
+  const int64_t n = (int64_t)a.batch * a.length;
+  const int rank = blockIdx.x % a.ctas, first = blockIdx.x / a.ctas, row_step = gridDim.x / a.ctas;
+  const int active = a.counts[0];
+  Sums sums;
+  for (int64_t pos = first; pos < n; pos += row_step) {
+    const int64_t r = a.order[pos];
+    if (pos >= active) {
+      if (a.ctas > 1) cluster_wait();
+      if (rank == 0 && threadIdx.x == 0) a.logp[r] = 0.f;
+      continue;
+    }
+    const T *x = logits + rows.offset(r);
+    const Slice<T> sl(x, a.vocab, rank, a.ctas);
+    Soft st;
+    add_range<T, false, kThreads, true>(st, sl.vecs() + sl.lo, sl.hi - sl.lo, a.c, threadIdx.x);
+    const int e = sl.edge(threadIdx.x);
+    if (e >= 0) add<false>(st, Elem<T>::to_f32(x[e]), a.c);
+    st = row_join<false>(st, a.c, red, rank, a.ctas);
+    if (rank == 0 && threadIdx.x == 0) token_result(a, token_in(a, x, r), st, r, sums);
+    if (a.ctas == 1) __syncthreads();  // every thread has read the warps' sums
+  }
+  if (rank == 0) finish<kThreads>(a, sums, first, row_step);
+}
+
+// A row without a weight: a gradient of zeros.
+template <typename T, int NT>
+__device__ __forceinline__ void zero_row(const PolicyArgs &a, T *grad, int64_t r, int tid) {
+  T *out = grad + r * (int64_t)a.vocab;
+  const Slice<T> sl(out, a.vocab, 0, 1);
+  uint4 *o = reinterpret_cast<uint4 *>(out + sl.head);
+#pragma unroll 4
+  for (int v = tid; v < sl.hi; v += NT) __stcs(o + v, make_uint4(0, 0, 0, 0));
+  const int e = sl.edge(tid);
+  if (e >= 0) out[e] = from_f32<T>(0.f);
+  if (tid == 0) a.logp[r] = 0.f;
+}
+
+// The loss and its gradient where a row fits in the registers of NT threads (a
+// warp, of which a block has W, or a block), NV vectors each: loaded once,
+// summed and turned into its gradient in place. The groups of threads take rows
+// in turn; several on an SM overlap their phases.
+template <typename T, int NT, int NV, int W, int PerSm>
+__global__ void __launch_bounds__(NT * W, PerSm)
+policy_row_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
+  static_assert(NT == 32 || W == 1, "several rows per block: one warp each");
+  __shared__ float2 part[NT / 32];
+  __shared__ RowResult result[W];
+  __shared__ Sums sums_s[W];
+  const int tid = threadIdx.x % NT, group = threadIdx.x / NT, lane = tid & 31, warp = tid >> 5;
+  const int64_t n = (int64_t)a.batch * a.length, step = (int64_t)gridDim.x * W;
+  const int active = a.counts[0];
+  auto sync = [] {
+    if (NT == 32)
+      __syncwarp();
+    else
+      __syncthreads();
+  };
+  Sums sums;
+  int64_t pos = (int64_t)blockIdx.x * W + group;
+  for (; pos < active; pos += step) {
+    const int64_t r = a.order[pos];
+    const T *x = logits + rows.offset(r);
+    const Slice<T> sl(x, a.vocab, 0, 1);
+    uint4 v[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (tid + j * NT < sl.hi) v[j] = __ldg(sl.vecs() + tid + j * NT);
+    TokenIn t;
+    if (tid == 0) t = token_in(a, x, r);
+    Soft st;
+#pragma unroll
+    for (int j = 0; j < NV; j += kUnroll) {
+      if (tid + (j + kUnroll - 1) * NT < sl.hi) {
+        const uint4 q[kUnroll] = {v[j], v[j + 1], v[j + 2], v[j + 3]};
+        add_vecs<T, false, kUnroll>(st, q, a.c);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (tid + (j + u) * NT < sl.hi) {
+            const uint4 q[1] = {v[j + u]};
+            add_vecs<T, false, 1>(st, q, a.c);
+          }
+      }
+    }
+    const int e = sl.edge(tid);
+    if (e >= 0) add<false>(st, Elem<T>::to_f32(x[e]), a.c);
+    __syncwarp();
+    warp_join<false>(st, a.c);
+    if (NT > 32) {
+      if (lane == 0) part[warp] = make_float2(st.m, st.s);
+      __syncthreads();
+      if (warp == 0) {
+        st = Soft();
+        if (lane < NT / 32) {
+          st.m = part[lane].x;
+          st.s = part[lane].y;
+        }
+        warp_join<false>(st, a.c);
+      }
+    }
+    if (tid == 0) result[group] = token_result(a, t, st, r, sums);
+    sync();
+    const RowResult res = result[group];
+    const Slope g{res.m, a.c, res.k, 0.f, res.slope, res.tok};
+    T *out = grad + r * (int64_t)a.vocab;
+    if ((reinterpret_cast<uintptr_t>(out + sl.head) & 15) == 0) {
+      uint4 *o = reinterpret_cast<uint4 *>(out + sl.head);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (tid + j * NT < sl.hi) __stcs(o + tid + j * NT, grad_vec<T, false>(g, v[j]));
+      const int64_t k = g.tok - sl.head;  // the token's share, from the thread that stored its vector
+      if (k >= 0 && k < (int64_t)sl.hi * Slice<T>::kV && (int)(k / Slice<T>::kV) % NT == tid)
+        out[g.tok] = from_f32<T>(grad_of<false>(g, Elem<T>::to_f32(x[g.tok]), (int)g.tok));
+    } else {
+      grad_range<T, false, NT>(sl, g, out, sl.vecs(), 0, sl.hi, tid);
+    }
+    grad_edge<T, false>(sl, g, out, tid);
+    sync();  // the results may be overwritten
+  }
+  for (; pos < n; pos += step) zero_row<T, NT>(a, grad, a.order[pos], tid);
+  if (W > 1) {
+    if (tid == 0) sums_s[group] = sums;
     __syncthreads();
-    if (tid < o)
-      for (int j = 0; j < 3; ++j) sums[j][tid] += sums[j][tid + o];
+    if (threadIdx.x == 0)
+      for (int i = 1; i < W; ++i) {
+        sums.loss += sums_s[i].loss;
+        sums.kl += sums_s[i].kl;
+        sums.clipped += sums_s[i].clipped;
+      }
   }
+  finish<NT * W>(a, sums, blockIdx.x, gridDim.x);
+}
+
+// The loss and its gradient, a persistent grid; a CTA takes every gridDim-th
+// row. The row is read from HBM once: its first K chunks (of kUnroll vectors per
+// thread) are copied to shared memory, the rest is streamed to the sums and read
+// again, from L2, for the gradient. The producer warp refills a chunk with the next
+// row's as soon as its gradient has gone out, and the consumers add the refilled
+// chunks up one chunk behind: reads, writes and arithmetic of two rows go on
+// together, and only the join of a row's sums stands alone.
+template <int NT, int K>
+struct GradShared {
+  uint64_t full[K], empty[K];  // a chunk has landed, has been used by every warp
+  uint64_t info;                           // token inputs are there
+  TokenIn token[2];
+  float2 part[NT / 32];
+  RowResult result;
+};
+
+template <typename T, int NT, int K, int PerSm>
+__global__ void __launch_bounds__(NT + 32, PerSm)
+policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
+  extern __shared__ __align__(16) uint8_t held_raw[];
+  __shared__ GradShared<NT, K> sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t n = (int64_t)a.batch * a.length;
+  const int active = a.counts[0];
+  uint4 *const hv = reinterpret_cast<uint4 *>(held_raw);
   if (tid == 0) {
-    const double count = max(1, a.counts[0]);
-    a.out[0] = (float)sums[0][0];
-    a.out[1] = (float)(sums[1][0] / count);
-    a.out[2] = (float)(sums[2][0] / count);
+    for (int k = 0; k < K; ++k) {
+      mbar_init(&sh.full[k], 1);
+      mbar_init(&sh.empty[k], NT / 32);
+    }
+    mbar_init(&sh.info, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  __syncthreads();
+  auto chunk = [](int held, int k) { return min(held, k * NT * kUnroll); };
+  bool ok = true;
+  Sums sums;
+
+  if (warp == NT / 32) {
+    // producer
+    if (lane == 0) {
+      int it = 0;
+      for (int64_t pos = blockIdx.x; pos < active; pos += gridDim.x, ++it) {
+        const int64_t r = a.order[pos];
+        const T *x = logits + rows.offset(r);
+        const Slice<T> sl(x, a.vocab, 0, 1);
+        const int held = min(sl.hi, a.hold);
+        for (int k = 0; k < K; ++k) {
+          if (it > 0) ok = mbar_wait_bounded(&sh.empty[k], (it - 1) & 1) && ok;
+          const int c0 = chunk(held, k), bytes = (chunk(held, k + 1) - c0) * 16;
+          mbar_expect(&sh.full[k], bytes);
+          if (bytes > 0)
+            asm volatile(
+                "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                    smem_u32(hv + c0)),
+                "l"(sl.vecs() + c0), "r"(bytes), "r"(smem_u32(&sh.full[k]))
+                : "memory");
+        }
+        // slot it & 1 was last read for row it - 2, before any chunk of row it - 1 was free
+        sh.token[it & 1] = token_in(a, x, r);
+        mbar_arrive(&sh.info);
+      }
+    }
+    __syncwarp();
+  } else {
+    // this thread's part of chunk k of the it-th row of this CTA
+    auto sum_chunk = [&](Soft &st, int held, int k, int it) {
+      const int c0 = chunk(held, k), c1 = chunk(held, k + 1);
+      ok = mbar_wait_bounded(&sh.full[k], it & 1) && ok;
+      add_range<T, false, NT, false>(st, hv + c0, c1 - c0, a.c, tid);
+    };
+    auto sum_rest = [&](Soft &st, const Slice<T> &sl, int held) {
+      add_range<T, false, NT, true>(st, sl.vecs() + held, sl.hi - held, a.c, tid);
+      const int e = sl.edge(tid);
+      if (e >= 0) add<false>(st, Elem<T>::to_f32(sl.x[e]), a.c);
+    };
+    int it = 0;
+    int64_t pos = blockIdx.x, r = a.order[pos];
+    Soft st;
+    if (pos < active) {
+      const Slice<T> sl(logits + rows.offset(r), a.vocab, 0, 1);
+      const int held = min(sl.hi, a.hold);
+      sum_rest(st, sl, held);
+      for (int k = 0; k < K; ++k) sum_chunk(st, held, k, 0);
+    }
+    for (; pos < active; pos += gridDim.x, ++it) {
+      const bool more = pos + gridDim.x < active;
+      const int64_t next = more ? a.order[pos + gridDim.x] : r;
+      // the row's sums, joined over the block
+      warp_join<false>(st, a.c);
+      if (lane == 0) sh.part[warp] = make_float2(st.m, st.s);
+      bar_sync<NT>();
+      if (warp == 0) {
+        st = Soft();
+        if (lane < NT / 32) {
+          st.m = sh.part[lane].x;
+          st.s = sh.part[lane].y;
+        }
+        warp_join<false>(st, a.c);
+        ok = mbar_wait_bounded(&sh.info, it & 1) && ok;
+        if (lane == 0) sh.result = token_result(a, sh.token[it & 1], st, r, sums);
+        __syncwarp();
+      }
+      bar_sync<NT>();
+      const Slope g{sh.result.m, a.c, sh.result.k, 0.f, sh.result.slope, sh.result.tok};
+      const Slice<T> sl(logits + rows.offset(r), a.vocab, 0, 1), sn(logits + rows.offset(next), a.vocab, 0, 1);
+      const int held = min(sl.hi, a.hold), held_n = min(sn.hi, a.hold);
+      T *out = grad + r * (int64_t)a.vocab;
+      st = Soft();
+      for (int k = 0; k < K; ++k) {
+        const int c0 = chunk(held, k), c1 = chunk(held, k + 1);
+        grad_range<T, false, NT>(sl, g, out, hv + c0, c0, c1, tid);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.empty[k]);
+        if (more && k > 0) sum_chunk(st, held_n, k - 1, it + 1);
+      }
+      grad_range<T, false, NT>(sl, g, out, sl.vecs() + held, held, sl.hi, tid);
+      grad_edge<T, false>(sl, g, out, tid);
+      if (more) {
+        sum_rest(st, sn, held_n);
+        sum_chunk(st, held_n, K - 1, it + 1);
+      }
+      r = next;
+    }
+    for (; pos < n; pos += gridDim.x) zero_row<T, NT>(a, grad, a.order[pos], tid);
+  }
+  if (!ok) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
+  __syncthreads();
+  finish<NT + 32>(a, sums, blockIdx.x, gridDim.x);
 }
 
 // grad *= *upstream, nothing where it is 1
@@ -606,19 +934,18 @@ int row_ctas(int64_t rows, int64_t row_bytes, int64_t most) {
   return ctas;
 }
 
+// Rows of up to 16 KB go to a warp each where that gives every SM eight of them.
+bool warp_rows(int64_t rows, int64_t row_bytes) { return row_bytes <= 16 * 1024 && rows >= 8 * 148; }
+
 template <typename K, typename... Args>
-int launch_rows(const char *what, K kern, int64_t rows, int ctas, size_t smem, void *stream, Args... args) {
+int launch_rows(const char *what, K kern, int64_t rows, int ctas, void *stream, Args... args) {
   if (rows * ctas > INT32_MAX) {
     set_error_detail("%s: %lld rows are too many for one call", what, (long long)rows);
     return PKV_ERR_UNSUPPORTED;
   }
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return check_launch(what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * ctas));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = reinterpret_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -629,6 +956,40 @@ int launch_rows(const char *what, K kern, int64_t rows, int ctas, size_t smem, v
   cfg.numAttrs = ctas > 1 ? 1 : 0;
   (void)cudaLaunchKernelEx(&cfg, kern, args...);
   return check_launch(what);
+}
+
+template <typename T, int NT, int NV, int W, int PerSm>
+int launch_row(const T *logits, Rows rows, T *grad, const PolicyArgs &a, void *stream) {
+  static_assert(148 * PerSm <= kMaxBlocks, "blocks with sums");
+  const unsigned blocks = (unsigned)std::min<int64_t>(((int64_t)a.batch * a.length - 1) / W + 1, 148 * PerSm);
+  policy_row_kernel<T, NT, NV, W, PerSm>
+      <<<blocks, NT * W, 0, reinterpret_cast<cudaStream_t>(stream)>>>(logits, rows, grad, a);
+  return check_launch("pkv_policy_loss");
+}
+
+template <typename T, int NT, int K, int PerSm>
+int launch_held(const T *logits, Rows rows, T *grad, PolicyArgs a, void *stream) {
+  a.hold = K * NT * kUnroll;
+  const int smem = a.hold * 16;
+  auto kern = policy_grad_kernel<T, NT, K, PerSm>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return check_launch("cudaFuncSetAttribute(policy_grad)");
+  const unsigned blocks = (unsigned)std::min<int64_t>((int64_t)a.batch * a.length, 148 * PerSm);
+  kern<<<blocks, NT + 32, smem, reinterpret_cast<cudaStream_t>(stream)>>>(logits, rows, grad, a);
+  return check_launch("pkv_policy_loss");
+}
+
+// By what holds a row: a warp's registers, a small or a larger block's, or shared memory.
+template <typename T>
+int launch_grad(const T *logits, Rows rows, T *grad, const PolicyArgs &a, void *stream) {
+  const int64_t bytes = (int64_t)a.vocab * sizeof(T);
+  if (bytes <= 32 * 16 * 16) return launch_row<T, 32, 16, 4, 4>(logits, rows, grad, a, stream);
+  if (bytes <= 128 * 16 * 16) return launch_row<T, 128, 16, 1, 4>(logits, rows, grad, a, stream);
+  if (bytes <= 256 * 16 * 16) return launch_row<T, 256, 16, 1, 2>(logits, rows, grad, a, stream);
+  // two blocks on an SM hold 96 KB each: 304 KB rows take 535 us for 4096 in one block and 568 in two, 100 KB rows
+  // 254 and 182 us for 4096, 200 KB rows 185 and 174 us for 2048
+  if (bytes <= 200 * 1024) return launch_held<T, 384, 4, 2>(logits, rows, grad, a, stream);
+  return launch_held<T, 768, 4, 1>(logits, rows, grad, a, stream);
 }
 
 bool bad_logits(const char *fn, const void *logits, int32_t dtype, int64_t rows, int32_t vocab, int32_t inner,
@@ -658,13 +1019,18 @@ extern "C" int pkv_token_logprobs(const void *logits, int32_t dtype, const int64
     return PKV_ERR_INVALID_ARG;
   }
   const Rows rw{outer_stride, row_stride, inner};
-  const int ctas = row_ctas(rows, (int64_t)vocab * dtype_size(dtype), INT64_MAX / kMaxCluster);
-  const float inv_t = 1.f / temperature, c = (float)(kLog2e / temperature);
-  float2 *s2 = reinterpret_cast<float2 *>(stats);
-  PKV_BY_DTYPE(dtype, return launch_rows("pkv_token_logprobs",
-                                         entropy ? logprob_kernel<T, true> : logprob_kernel<T, false>, rows, ctas, 0,
-                                         stream, (const T *)logits, rw, tokens, vocab, ctas, inv_t, c, logprobs,
-                                         entropy, s2, status))
+  const int64_t bytes = (int64_t)vocab * dtype_size(dtype);
+  LogprobArgs p{tokens, logprobs, entropy, reinterpret_cast<float2 *>(stats), status, rows, vocab,
+                row_ctas(rows, bytes, INT64_MAX / kMaxCluster), 1.f / temperature, (float)(kLog2e / temperature)};
+  if (warp_rows(rows, bytes)) {
+    PKV_BY_DTYPE(dtype, return launch_rows("pkv_token_logprobs",
+                                           entropy ? logprob_warp_kernel<T, true> : logprob_warp_kernel<T, false>,
+                                           (rows - 1) / kWarps + 1, 1, stream, (const T *)logits, rw, p))
+  } else {
+    PKV_BY_DTYPE(dtype, return launch_rows("pkv_token_logprobs",
+                                           entropy ? logprob_kernel<T, true> : logprob_kernel<T, false>, rows, p.ctas,
+                                           stream, (const T *)logits, rw, p))
+  }
   return PKV_ERR_UNSUPPORTED;
 }
 
@@ -682,20 +1048,31 @@ extern "C" int pkv_token_logprobs_grad(const void *logits, int32_t dtype, const 
     return PKV_ERR_INVALID_ARG;
   }
   const Rows rw{outer_stride, row_stride, inner};
-  const int ctas = row_ctas(rows, (int64_t)vocab * dtype_size(dtype), 64 * 1024);
-  const float inv_t = 1.f / temperature, c = (float)(kLog2e / temperature);
-  const float2 *s2 = reinterpret_cast<const float2 *>(stats);
-  PKV_BY_DTYPE(dtype, return launch_rows("pkv_token_logprobs_grad",
-                                         d_entropy ? logprob_grad_kernel<T, true> : logprob_grad_kernel<T, false>, rows,
-                                         ctas, 0, stream, (const T *)logits, rw, tokens, vocab, ctas, inv_t, c, s2,
-                                         entropy, d_logprobs, d_entropy, (T *)d_logits))
+  const int64_t bytes = (int64_t)vocab * dtype_size(dtype);
+  LogprobArgs p{tokens, nullptr, const_cast<float *>(entropy), reinterpret_cast<float2 *>(const_cast<float *>(stats)),
+                nullptr, rows, vocab, 1, 1.f / temperature, (float)(kLog2e / temperature)};
+  if (warp_rows(rows, bytes)) {
+    PKV_BY_DTYPE(dtype, return launch_rows("pkv_token_logprobs_grad",
+                                           d_entropy ? logprob_grad_kernel<T, true, 32>
+                                                     : logprob_grad_kernel<T, false, 32>,
+                                           (rows - 1) / kWarps + 1, 1, stream, (const T *)logits, rw, p, d_logprobs,
+                                           d_entropy, (T *)d_logits))
+  } else {
+    // shares of 64 KB, and of as little as 4 KB where the rows are few; they do not talk to each other
+    p.ctas = row_ctas(rows, bytes, 64 * 1024);
+    PKV_BY_DTYPE(dtype, return launch_rows("pkv_token_logprobs_grad",
+                                           d_entropy ? logprob_grad_kernel<T, true, kThreads>
+                                                     : logprob_grad_kernel<T, false, kThreads>,
+                                           rows * p.ctas, 1, stream, (const T *)logits, rw, p, d_logprobs, d_entropy,
+                                           (T *)d_logits))
+  }
   return PKV_ERR_UNSUPPORTED;
 }
 
 extern "C" size_t pkv_policy_loss_workspace_size(int32_t batch, int32_t length) {
   if (batch < 0 || length < 0 || (int64_t)batch * length > INT32_MAX) return 0;
-  // terms (16 bytes), weight, order (4 each) per token; two counters; a count per sequence
-  return 16 + (size_t)batch * length * 24 + ((size_t)batch + 1) * 4;
+  // the blocks' sums, two counters, an index per token, a count per sequence
+  return kMaxBlocks * 24 + 16 + ((size_t)batch * length + batch + 1) * 4;
 }
 
 extern "C" int pkv_policy_loss(const void *logits, int32_t dtype, const int64_t *tokens, const float *old_logprobs,
@@ -732,11 +1109,10 @@ extern "C" int pkv_policy_loss(const void *logits, int32_t dtype, const int64_t 
   a.out = out;
   a.logp = logprobs;
   uint8_t *ws = static_cast<uint8_t *>(workspace);
-  a.counts = reinterpret_cast<int32_t *>(ws);
-  a.terms = reinterpret_cast<float4 *>(ws + 16);
-  a.weight = reinterpret_cast<float *>(ws + 16 + 16 * rows);
-  a.order = reinterpret_cast<int32_t *>(ws + 16 + 20 * rows);
-  a.before = reinterpret_cast<int32_t *>(ws + 16 + 24 * rows);
+  a.partial = reinterpret_cast<double *>(ws);
+  a.counts = reinterpret_cast<int32_t *>(ws + kMaxBlocks * 24);
+  a.order = a.counts + 4;
+  a.before = a.order + rows;
   a.status = status;
   a.adv_b = adv_stride_b;
   a.adv_t = adv_stride_t;
@@ -751,16 +1127,18 @@ extern "C" int pkv_policy_loss(const void *logits, int32_t dtype, const int64_t 
   a.kl_coef = kl_coef;
   const Rows rw{batch_stride, row_stride, length};
   const int64_t row_bytes = (int64_t)vocab * dtype_size(dtype);
-  a.ctas = row_ctas(rows, row_bytes, d_logits ? kHoldTarget : INT64_MAX / kMaxCluster);
-  // a slice has at most one vector more than its even share
-  const int64_t share = row_bytes / 16 / a.ctas + 1;
-  a.hold = d_logits ? (int)std::min<int64_t>(share, kHoldMost / 16) : 0;
-  policy_prep_kernel<<<1, kPrepThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+  a.ctas = row_ctas(rows, row_bytes, INT64_MAX / kMaxCluster);
+  policy_prep_kernel<<<(unsigned)((rows - 1) / kPrepThreads + 1), kPrepThreads, 0,
+                       reinterpret_cast<cudaStream_t>(stream)>>>(a);
   const int rc = check_launch("policy_prep_kernel");
   if (rc) return rc;
-  PKV_BY_DTYPE(dtype, return launch_rows("pkv_policy_loss", d_logits ? policy_kernel<T, true> : policy_kernel<T, false>,
-                                         rows, a.ctas, (size_t)a.hold * 16, stream, (const T *)logits, rw,
-                                         (T *)d_logits, a))
+  if (d_logits) {
+    PKV_BY_DTYPE(dtype, return launch_grad((const T *)logits, rw, (T *)d_logits, a, stream))
+  } else {
+    PKV_BY_DTYPE(dtype, return launch_rows("pkv_policy_loss", policy_kernel<T>,
+                                           std::min<int64_t>(rows, kMaxBlocks), a.ctas, stream, (const T *)logits, rw,
+                                           a))
+  }
   return PKV_ERR_UNSUPPORTED;
 }
 

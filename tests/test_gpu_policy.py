@@ -45,7 +45,8 @@ def _check_grad(got, want, bulk):
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("rows,vocab,temperature", [(1, 1, 1.0), (1, 151936, 0.7), (3, 2, 1.0), (5, 7, 1.3),
                                                     (4, 1000, 1.0), (9, 1001, 0.7), (40, 32003, 1.0),
-                                                    (200, 151936, 1.0), (2, 300007, 1.0), (2000, 100, 1.0)])
+                                                    (200, 151936, 1.0), (2, 300007, 1.0), (2000, 100, 1.0),
+                                                    (1201, 2003, 1.0)])
 def test_token_logprobs_and_gradient(rows, vocab, temperature, dtype):
     logits = _logits((rows, vocab), dtype, rows + vocab).requires_grad_()
     tokens = torch.randint(0, vocab, (rows,), device="cuda")
@@ -222,7 +223,8 @@ def _batch(batch, length, vocab, dtype, seed, kl=True, per_token=False, temperat
 @pytest.mark.parametrize("batch,length,vocab,reduction,temperature", [
     (1, 1, 1, "token", 1.0), (1, 1, 151936, "sequence", 1.0), (2, 9, 1000, "token", 1.0),
     (3, 5, 1003, "sequence", 0.7), (4, 33, 129, "sum", 1.3), (8, 40, 32003, "sequence", 1.0),
-    (2, 100, 151936, "token", 1.0), (1, 1500, 64, "sequence", 1.0), (7, 3, 200001, "sum", 1.0)])
+    (2, 100, 151936, "token", 1.0), (1, 1500, 64, "sequence", 1.0), (7, 3, 200001, "sum", 1.0),
+    (3, 70, 9001, "token", 1.0), (2, 200, 45001, "sequence", 1.0)])
 def test_policy_loss(batch, length, vocab, reduction, temperature, dtype):
     kl, per_token = bool((batch + length) % 2), length % 3 == 0
     logits, tokens, old, adv, mask, ref = _batch(batch, length, vocab, dtype, vocab, kl, per_token, temperature)
