@@ -34,52 +34,162 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-constexpr int kNormThreads = 256;
+// 16 bytes as N fp32 values, and back.
+template <typename T> struct alignas(16) Vec16 {
+  static constexpr int kN = 16 / (int)sizeof(T);
+  T e[kN];
+};
+
+__device__ __forceinline__ float sum_block(float v, float *red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.f;
+  for (int k = 0; k < (int)blockDim.x / 32; ++k) v += red[k];
+  return v;
+}
+
+struct NormArgs {
+  const void *x, *res, *w;
+  void *sum;
+  uint8_t *q;
+  float *scales;
+  int64_t xs, rs, ss, qs, cs;
+  int hidden;
+  float eps;
+};
+
+// One block per row, NV vectors of 16 bytes per thread, the row held in
+// registers between the sum of squares and the quotient: x, the residual and
+// their sum cross HBM once. A group of 128 values is the vectors of 32 (fp32)
+// or 16 neighbouring lanes. Bound by HBM.
+template <typename T, int NV, bool Res>
+__global__ void __launch_bounds__(NV == 4 ? 512 : 1024) norm_fp8_kernel(NormArgs a) {
+  using V = Vec16<T>;
+  constexpr int N = V::kN, kLanes = kGroup / N;
+  __shared__ float red[32];
+  const int64_t b = blockIdx.x;
+  const int tid = threadIdx.x, nt = blockDim.x, nv = a.hidden / N;
+  const V *x = reinterpret_cast<const V *>(reinterpret_cast<const T *>(a.x) + b * a.xs);
+  const V *res = reinterpret_cast<const V *>(reinterpret_cast<const T *>(a.res) + b * a.rs);
+  V *sum = reinterpret_cast<V *>(reinterpret_cast<T *>(a.sum) + b * a.ss);
+  const V *w = reinterpret_cast<const V *>(a.w);
+  V xv[NV], rv[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if (tid + j * nt < nv) {
+      // read for the last time: what is read again is their sum
+      *reinterpret_cast<uint4 *>(&xv[j]) = __ldcs(reinterpret_cast<const uint4 *>(x + tid + j * nt));
+      if (Res) *reinterpret_cast<uint4 *>(&rv[j]) = __ldcs(reinterpret_cast<const uint4 *>(res + tid + j * nt));
+    }
+  float s[NV][N], acc = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const bool in = tid + j * nt < nv;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      s[j][e] = in ? Elem<T>::to_f32(xv[j].e[e]) : 0.f;
+      if (Res && in) {
+        s[j][e] += Elem<T>::to_f32(rv[j].e[e]);
+        xv[j].e[e] = from_f32<T>(s[j][e]);
+      }
+      acc += s[j][e] * s[j][e];
+    }
+    if (Res && in) sum[tid + j * nt] = xv[j];
+  }
+  const float r = rsqrtf(sum_block(acc, red) / (float)a.hidden + a.eps);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int i = tid + j * nt;
+    const bool in = i < nv;
+    float amax = 0.f;
+    if (in) {
+      const V wv = w[i];
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        s[j][e] *= r * Elem<T>::to_f32(wv.e[e]);
+        amax = max_nan(amax, fabsf(s[j][e]));
+      }
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const float scale = group_scale(amax), inv = 1.f / scale;
+    if (!in) continue;
+    if (i % kLanes == 0) a.scales[b * a.cs + i / kLanes] = scale;
+    uint32_t o[N / 4];
+#pragma unroll
+    for (int e = 0; e < N; e += 4)
+      o[e / 4] = e4m3x2(s[j][e] * inv, s[j][e + 1] * inv) |
+                 ((uint32_t)e4m3x2(s[j][e + 2] * inv, s[j][e + 3] * inv) << 16);
+    uint8_t *q = a.q + b * a.qs + (int64_t)i * N;
+    if (N == 8)
+      *reinterpret_cast<uint2 *>(q) = make_uint2(o[0], o[N / 4 - 1]);
+    else
+      *reinterpret_cast<uint32_t *>(q) = o[0];
+  }
+}
+
+// Rows of any length and alignment, element by element (the second read: L1/L2).
+constexpr int kAnyThreads = 256;
 
 template <typename T>
-__global__ void __launch_bounds__(kNormThreads)
-norm_fp8_kernel(const T *x, const T *res, const T *w, T *sum_out, uint8_t *q, float *scales, int H, int64_t xs,
-                int64_t rs, int64_t ss, int64_t qs, int64_t cs, float eps) {
-  __shared__ float red[kNormThreads / 32];
+__global__ void __launch_bounds__(kAnyThreads) norm_fp8_any_kernel(NormArgs a) {
+  __shared__ float red[32];
   const int64_t b = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  float acc = 0.f;
-  for (int i = tid; i < H; i += kNormThreads) {
-    float s = Elem<T>::to_f32(x[b * xs + i]);
-    if (res != nullptr) {
-      s += Elem<T>::to_f32(res[b * rs + i]);
-      sum_out[b * ss + i] = from_f32<T>(s);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, H = a.hidden;
+  const T *x = reinterpret_cast<const T *>(a.x) + b * a.xs;
+  const T *res = a.res != nullptr ? reinterpret_cast<const T *>(a.res) + b * a.rs : nullptr;
+  T *sum = reinterpret_cast<T *>(a.sum) + b * a.ss;
+  const T *w = reinterpret_cast<const T *>(a.w);
+  // a warp's groups in both passes: what it reads again it has read itself, before it stored the sum
+  constexpr int kHeld = 4;  // groups per warp that stay in registers
+  float held[kHeld][4], acc = 0.f;
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = (warp + j * (kAnyThreads / 32)) * kGroup + lane + 32 * e;
+      held[j][e] = 0.f;
+      if (i < H) {
+        held[j][e] = Elem<T>::to_f32(x[i]) + (res != nullptr ? Elem<T>::to_f32(res[i]) : 0.f);
+        acc += held[j][e] * held[j][e];
+      }
     }
-    acc += s * s;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  if (lane == 0) red[warp] = acc;
-  __syncthreads();
-  float tot = 0.f;
-#pragma unroll
-  for (int k = 0; k < kNormThreads / 32; ++k) tot += red[k];
-  const float r = rsqrtf(tot / (float)H + eps);
-  // one warp per group, 4 values per lane
-  for (int g = warp; g * kGroup < H; g += kNormThreads / 32) {
+  for (int g = warp + kHeld * (kAnyThreads / 32); g * kGroup < H; g += kAnyThreads / 32)
+    for (int i = g * kGroup + lane; i < min(H, (g + 1) * kGroup); i += 32) {
+      const float s = Elem<T>::to_f32(x[i]) + (res != nullptr ? Elem<T>::to_f32(res[i]) : 0.f);
+      acc += s * s;
+    }
+  const float r = rsqrtf(sum_block(acc, red) / (float)H + a.eps);
+  auto write = [&](int g, const float (&s)[4]) {
     float y[4], amax = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int i = g * kGroup + lane * 4 + e;
-      y[e] = 0.f;
-      if (i < H) {
-        float s = Elem<T>::to_f32(x[b * xs + i]);
-        if (res != nullptr) s += Elem<T>::to_f32(res[b * rs + i]);
-        y[e] = s * r * Elem<T>::to_f32(w[i]);
-      }
+      const int i = g * kGroup + lane + 32 * e;
+      y[e] = i < H ? s[e] * (r * Elem<T>::to_f32(w[i])) : 0.f;
       amax = max_nan(amax, fabsf(y[e]));
+      if (res != nullptr && i < H) sum[i] = from_f32<T>(s[e]);
     }
     const float scale = group_scale(warp_max(amax)), inv = 1.f / scale;
-    if (lane == 0) scales[b * cs + g] = scale;
-    const uint32_t p = e4m3x2(y[0] * inv, y[1] * inv) | ((uint32_t)e4m3x2(y[2] * inv, y[3] * inv) << 16);
+    if (lane == 0) a.scales[b * a.cs + g] = scale;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (g * kGroup + lane * 4 + e < H) q[b * qs + g * kGroup + lane * 4 + e] = (uint8_t)(p >> (8 * e));
+    for (int e = 0; e < 4; ++e) {
+      const int i = g * kGroup + lane + 32 * e;
+      if (i < H) a.q[b * a.qs + i] = (uint8_t)e4m3x2(y[e] * inv, 0.f);
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if ((warp + j * (kAnyThreads / 32)) * kGroup < H) write(warp + j * (kAnyThreads / 32), held[j]);
+  for (int g = warp + kHeld * (kAnyThreads / 32); g * kGroup < H; g += kAnyThreads / 32) {
+    float s[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = g * kGroup + lane + 32 * e;
+      s[e] = i < H ? Elem<T>::to_f32(x[i]) + (res != nullptr ? Elem<T>::to_f32(res[i]) : 0.f) : 0.f;
+    }
+    write(g, s);
   }
 }
 
@@ -129,9 +239,30 @@ extern "C" int pkv_add_rmsnorm_fp8(const void *x, const void *residual, const vo
   for (const void *p : ptrs)
     if (!aligned_to(p, es)) return PKV_ERR_ALIGNMENT;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  PKV_BY_DTYPE(dtype, (norm_fp8_kernel<T><<<rows, kNormThreads, 0, st>>>(
-                          (const T *)x, (const T *)residual, (const T *)weight, (T *)sum_out, (uint8_t *)q_out, scales,
-                          hidden, x_stride, residual_stride, sum_stride, q_stride, scale_stride, eps)))
+  const NormArgs a{x, residual, weight, sum_out, (uint8_t *)q_out, scales, x_stride, residual_stride, sum_stride,
+                   q_stride, scale_stride, hidden, eps};
+  // 16-byte vectors where every row begins on one; q's rows take the vectors' 8-bit images
+  const int n = 16 / es;
+  const int64_t strides[] = {x_stride, residual ? residual_stride : 0, sum_out ? sum_stride : 0};
+  bool vec = hidden % n == 0 && hidden / n <= 2 * 1024 && aligned_to(q_out, n) && q_stride % n == 0;
+  for (const void *p : ptrs) vec = vec && aligned_to(p, 16);
+  for (int64_t v : strides) vec = vec && v % n == 0;
+  if (!vec) {
+    PKV_BY_DTYPE(dtype, (norm_fp8_any_kernel<T><<<rows, kAnyThreads, 0, st>>>(a)))
+    return check_launch("pkv_add_rmsnorm_fp8");
+  }
+  // Few rows: one vector per thread, for the shortest chain. Many: four, for the most bytes in flight per
+  // register and the fewest blocks.
+  const int nv = hidden / n;
+  const int per = std::max(rows <= 2 * 148 ? 1 : rows <= 16 * 148 ? 2 : 4, nv > 1024 ? 2 : 1);
+  const int threads = ((nv + per - 1) / per + 31) / 32 * 32;
+  PKV_BY_DTYPE(dtype, {
+    auto k = residual ? (per == 1 ? norm_fp8_kernel<T, 1, true> : per == 2 ? norm_fp8_kernel<T, 2, true>
+                                                                            : norm_fp8_kernel<T, 4, true>)
+                      : (per == 1 ? norm_fp8_kernel<T, 1, false> : per == 2 ? norm_fp8_kernel<T, 2, false>
+                                                                             : norm_fp8_kernel<T, 4, false>);
+    k<<<rows, threads, 0, st>>>(a);
+  })
   return check_launch("pkv_add_rmsnorm_fp8");
 }
 

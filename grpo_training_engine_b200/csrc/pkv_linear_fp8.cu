@@ -10,13 +10,21 @@
 // of their own, and the epilogue warps add it, times the block's two scales,
 // to fp32 accumulators in registers while the tensor core fills the next.
 //
-// One CTA computes a 128-row by BN-column tile (or one split of its k):
+// A persistent grid; a CTA (G = 1), or a pair of CTAs on one MMA (G = 2, twice
+// the rows, each loading half of the columns), takes tiles of 128 G rows by BN
+// columns in turn:
 //   warp 0, one thread : TMA loads of 128-wide k blocks of x and W into an
 //                        S-stage shared-memory ring (128-byte swizzle)
-//   warp 1             : TMEM allocation; one thread issues the 4 MMAs (M 128,
-//                        N BN, K 32) of each block
-//   warps 2-9          : two warps per 32-lane TMEM group, half the columns
-//                        each: accumulate block by block, then store.
+//   warp 1             : TMEM allocation; one thread (of the pair's first CTA)
+//                        issues the 4 MMAs (M 128 G, N BN, K 32) of each block
+//   warp 2             : the products of the two scales for each row and block,
+//                        into a ring of their own: straight from global memory
+//                        every epilogue thread's load would be a line of its own
+//   warps 4-11         : two warps per 32-lane TMEM group, half of the columns
+//                        each: accumulate block by block, then store through
+//                        shared memory by TMA, while the next tile's blocks are
+//                        loaded and multiplied. They take the registers that the
+//                        first four warps give up.
 // With few rows the tiles of one weight matrix are split along k over the CTAs
 // of a cluster, which add their fp32 tiles in split order through distributed
 // shared memory, so results do not depend on timing.
@@ -33,8 +41,12 @@ namespace pkv {
 namespace {
 
 constexpr int kBM = 128, kBK = 128;  // tile rows; k values of a block, the span of one scale
-constexpr int kEpiWarps = 8, kThreads = 64 + 32 * kEpiWarps;
 constexpr int kMaxSplits = 8;        // a portable cluster
+constexpr int kFirstEpi = 4;         // first epilogue warp: its warpgroup is all epilogue
+constexpr int kEpiWarps = 8, kThreads = 32 * (kFirstEpi + kEpiWarps);
+// registers per thread: 384 threads start with 168 each, 64512 in all = 128 x 72 + 256 x 216
+constexpr int kRegsOther = 72, kRegsEpi = 216;
+constexpr int kScales = 8;           // k blocks whose scales are ready ahead
 
 struct Fp8Args {
   const float *xs, *ws;  // scales: rows of x, blocks of W
@@ -43,71 +55,165 @@ struct Fp8Args {
   int32_t *status;
   int64_t xs_stride, ws_stride, out_stride;
   int32_t rows, n, kblocks, tiles_m, tiles_n, splits;
+  int32_t tma_out;  // out can be stored by TMA: 16-byte aligned base and rows
   uint32_t max_polls;
 };
 
-// D[tmem] (+)= A[smem] B[smem]^T with e4m3 operands
+// D[tmem] (+)= A[smem] B[smem]^T with e4m3 operands, by one CTA or a pair
+template <int G>
 __device__ __forceinline__ void tc_mma_f8(uint32_t tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                           uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
-      : "memory");
+  if constexpr (G == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
 }
 
-// Instruction descriptor: fp32 accumulator, A and B e4m3 (0), both K-major, M 128, N n.
-__host__ __device__ constexpr uint32_t f8_idesc(int n) {
-  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+// Arrive on `bar` (of both CTAs of a pair) once every MMA issued before has completed.
+template <int G>
+__device__ __forceinline__ void tc_commit_group(uint64_t *bar) {
+  if constexpr (G == 1)
+    tc_commit(bar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+// TMA load into this CTA's shared memory that completes on a barrier of the
+// pair's first CTA (`bar`: its cluster address).
+template <int G>
+__device__ __forceinline__ void tma_load_group(void *dst, const CUtensorMap *map, int32_t x, int32_t y, uint32_t bar) {
+  if constexpr (G == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+// Bounded wait of a thread that others wait for in turn: it looks again at once.
+__device__ __forceinline__ bool mbar_wait_spin(uint64_t *bar, uint32_t parity, uint32_t max_polls) {
+  for (uint32_t i = 0; i < max_polls; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+
+// Instruction descriptor: fp32 accumulator, A and B e4m3 (0), both K-major, M m, N n.
+__host__ __device__ constexpr uint32_t f8_idesc(int m, int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// 32 columns of this thread's TMEM lane; the values are there after tmem_wait.
+__device__ __forceinline__ void tmem_ld_async(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr));
+}
+// Waits for this thread's loads; passing the registers through keeps their uses behind it.
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                 "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
+                 "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
+                 "+r"(v[30]), "+r"(v[31])
+               :
+               : "memory");
+}
+
+// acc += v * s, two columns per instruction
+template <int N>
+__device__ __forceinline__ void fma_cols(float2 (&acc)[N / 2], const uint32_t (&v)[N], float s) {
+#pragma unroll
+  for (int j = 0; j < N / 2; ++j)
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%0, %1};\n\t"
+        "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "+f"(acc[j].x), "+f"(acc[j].y)
+        : "r"(v[2 * j]), "r"(v[2 * j + 1]), "f"(s));
 }
 
 __device__ __forceinline__ uint32_t bits16(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 __device__ __forceinline__ uint32_t bits16(__half v) { return __half_as_ushort(v); }
 
-template <int BN, int S>
+template <int BN, int S, int G>
 struct Smem {
-  static constexpr int kA = kBM * kBK, kB = BN * kBK;  // one stage of x and of W, bytes
-  static constexpr int kBufs = BN <= 128 ? 4 : 2;      // TMEM buffers of BN fp32 columns
-  static constexpr uint32_t kCols = kBufs * BN;        // a power of two, at most 512
+  static constexpr int kA = kBM * kBK, kB = BN / G * kBK;  // one stage of x and of W, bytes
+  static constexpr int kBufs = 512 / BN;                   // TMEM buffers of BN fp32 columns: all 512 columns
+  static constexpr int kCW = BN / 2;                       // columns of an epilogue warp
+  static constexpr int kBlocks = (BN + 127) / 128;         // blocks of W's scales across a tile
   static constexpr size_t kW = (size_t)S * kA;
-  static constexpr size_t kFull = kW + (size_t)S * kB;
+  static constexpr size_t kOut = kW + (size_t)S * kB;      // 32 rows x kCW 16-bit results of each epilogue warp
+  static constexpr size_t kSc = kOut + (size_t)kEpiWarps * 32 * kCW * 2;  // [kScales][kBlocks][kBM] fp32
+  static constexpr size_t kFull = kSc + 4 * kScales * kBlocks * kBM;
   static constexpr size_t kEmpty = kFull + 8 * S;
   static constexpr size_t kAccFull = kEmpty + 8 * S;
   static constexpr size_t kAccEmpty = kAccFull + 8 * kBufs;
-  static constexpr size_t kDone = kAccEmpty + 8 * kBufs;
+  static constexpr size_t kScFull = kAccEmpty + 8 * kBufs;
+  static constexpr size_t kScEmpty = kScFull + 8 * kScales;
+  static constexpr size_t kDone = kScEmpty + 8 * kScales;
   static constexpr size_t kTmem = kDone + 8;
   static constexpr size_t kBytes = kTmem + 8 + 1024;  // + alignment slack
 };
 
-// NC results of one row from column col on: bias, rounding, store.
+// NC results of one row, rounded.
+template <typename T, int NC>
+__device__ __forceinline__ void round_cols(const float *v, T (&o)[NC]) {
+#pragma unroll
+  for (int j = 0; j < NC; ++j) o[j] = from_f32<T>(v[j]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack_8(const T (&o)[8]) {
+  return make_uint4(bits16(o[0]) | (bits16(o[1]) << 16), bits16(o[2]) | (bits16(o[3]) << 16),
+                    bits16(o[4]) | (bits16(o[5]) << 16), bits16(o[6]) | (bits16(o[7]) << 16));
+}
+
+// ... and stored.
 template <typename T, int NC>
 __device__ __forceinline__ void store_cols(const Fp8Args &a, int row, int col, const float *v) {
   T *out = reinterpret_cast<T *>(a.out) + row * a.out_stride + col;
-  const T *bias = reinterpret_cast<const T *>(a.bias);
   T o[NC];
+  round_cols<T, NC>(v, o);
+  if constexpr (NC == 8) {
+    if (col + NC <= a.n && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+      *reinterpret_cast<uint4 *>(out) = pack_8(o);
+      return;
+    }
+  }
 #pragma unroll
   for (int j = 0; j < NC; ++j)
-    o[j] = from_f32<T>(bias != nullptr && col + j < a.n ? v[j] + Elem<T>::to_f32(bias[col + j]) : v[j]);
-  if (NC == 8 && col + NC <= a.n && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
-    uint4 w;
-    w.x = bits16(o[0]) | (bits16(o[1]) << 16);
-    w.y = bits16(o[2]) | (bits16(o[3]) << 16);
-    w.z = bits16(o[4]) | (bits16(o[5]) << 16);
-    w.w = bits16(o[6]) | (bits16(o[7]) << 16);
-    *reinterpret_cast<uint4 *>(out) = w;
-  } else {
-#pragma unroll
-    for (int j = 0; j < NC; ++j)
-      if (col + j < a.n) out[j] = o[j];
-  }
+    if (col + j < a.n) out[j] = o[j];
 }
 
-template <typename T, int BN, int S>
+template <typename T, int BN, int S, int G>
 __global__ void __launch_bounds__(kThreads, 1)
-linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, Fp8Args a) {
-  using L = Smem<BN, S>;
-  constexpr int NB = L::kBufs, kPart = BN / 2;  // columns of one epilogue warp
+linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
+                  const __grid_constant__ CUtensorMap to, Fp8Args a) {
+  using L = Smem<BN, S, G>;
+  constexpr int NB = L::kBufs, CW = L::kCW, ST = 32;
   extern __shared__ uint8_t raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   uint8_t *sa = smem, *sb = smem + L::kW;
@@ -116,11 +222,17 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
   uint64_t *acc_full = reinterpret_cast<uint64_t *>(smem + L::kAccFull);
   uint64_t *acc_empty = reinterpret_cast<uint64_t *>(smem + L::kAccEmpty);
   uint64_t *done = reinterpret_cast<uint64_t *>(smem + L::kDone);
+  uint64_t *sc_full = reinterpret_cast<uint64_t *>(smem + L::kScFull);
+  uint64_t *sc_empty = reinterpret_cast<uint64_t *>(smem + L::kScEmpty);
+  float *sc = reinterpret_cast<float *>(smem + L::kSc);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::kTmem);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = blockIdx.x / a.splits, split = blockIdx.x - tile * a.splits;
-  const int m0 = (tile % a.tiles_m) * kBM, n0 = (tile / a.tiles_m) * BN;
+  const int rank = G == 2 ? (int)(blockIdx.x & 1) : 0;  // in the pair
+  const int split = G == 1 ? (int)(blockIdx.x % a.splits) : 0;
+  const int first = G == 2 ? (int)(blockIdx.x >> 1) : (int)(blockIdx.x / a.splits);
+  const int step = G == 2 ? (int)(gridDim.x >> 1) : (int)(gridDim.x / a.splits);
+  const int tiles = a.tiles_m * a.tiles_n;
   const int kb0 = (int)((int64_t)split * a.kblocks / a.splits);
   const int nkb = (int)((int64_t)(split + 1) * a.kblocks / a.splits) - kb0;  // >= 1
 
@@ -131,117 +243,259 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
     }
     for (int s = 0; s < NB; ++s) {
       mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], kEpiWarps);
+      mbar_init(&acc_empty[s], kEpiWarps * G);
+    }
+    for (int s = 0; s < kScales; ++s) {
+      mbar_init(&sc_full[s], 1);
+      mbar_init(&sc_empty[s], kEpiWarps);
     }
     mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tx)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tw)) : "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(L::kCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (G == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(512)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(512)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (G == 2) cluster_sync();  // the pair's barriers and TMEM are ready in both CTAs
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  auto tile_m = [&](int t) { return (t % a.tiles_m) * (kBM * G) + rank * kBM; };  // this CTA's first row
+  auto tile_n = [&](int t) { return (t / a.tiles_m) * BN; };
 
-  if (warp == 0) {
-    if (lane == 0) {
-      int issued = 0;
-      for (int i = 0; i < nkb; ++i) {
-        const int s = i % S, use = i / S;
-        if (use > 0 && !mbar_wait_bounded(&empty[s], (use - 1) & 1, a.max_polls)) {
-          flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
-          break;
+  if (warp < kFirstEpi) {
+    if constexpr (G == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == 0) {
+      if (lane == 0) {
+        int i = 0, issued = 0;
+        bool ok = true;
+        for (int t = first; t < tiles && ok; t += step) {
+          const int m0 = tile_m(t), n0 = tile_n(t) + rank * (BN / G);
+          for (int k = 0; k < nkb; ++k, ++i) {
+            const int s = i % S, use = i / S;
+            if (use > 0 && !mbar_wait_spin(&empty[s], (use - 1) & 1, a.max_polls)) {
+              flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
+              ok = false;
+              break;
+            }
+            uint32_t bar = smem_u32(&full[s]);
+            if (G == 2) bar = map_cluster(bar, 0);
+            if (rank == 0) mbar_expect_tx(&full[s], G * (L::kA + L::kB));
+            tma_load_group<G>(sa + s * L::kA, &tx, (kb0 + k) * kBK, m0, bar);
+            tma_load_group<G>(sb + s * L::kB, &tw, (kb0 + k) * kBK, n0, bar);
+            ++issued;
+          }
         }
-        mbar_expect_tx(&full[s], L::kA + L::kB);
-        tma_load_2d(sa + s * L::kA, &tx, (kb0 + i) * kBK, m0, &full[s]);
-        tma_load_2d(sb + s * L::kB, &tw, (kb0 + i) * kBK, n0, &full[s]);
-        ++issued;
+        // the last load of each stage has landed before the shared memory goes away (in the pair's second
+        // CTA: the MMAs that read it are waited for)
+        if (rank == 0)
+          for (int j = issued > S ? issued - S : 0; j < issued; ++j)
+            if (!mbar_wait_spin(&full[j % S], (j / S) & 1, a.max_polls)) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
       }
-      // the last load of each stage has landed before the shared memory goes away
-      for (int i = issued > S ? issued - S : 0; i < issued; ++i)
-        if (!mbar_wait_bounded(&full[i % S], (i / S) & 1, a.max_polls)) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = f8_idesc(BN);
-      for (int i = 0; i < nkb; ++i) {
-        const int s = i % S, buf = i % NB, use = i / NB;
-        if ((use > 0 && !mbar_wait_bounded(&acc_empty[buf], (use - 1) & 1, a.max_polls)) ||
-            !mbar_wait_bounded(&full[s], (i / S) & 1, a.max_polls)) {
-          flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
-          break;
-        }
-        tc_fence_after();
-        const uint64_t ad = sw128_desc(sa + s * L::kA), bd = sw128_desc(sb + s * L::kB);
+    } else if (warp == 1) {
+      if (lane == 0 && rank == 0) {
+        constexpr uint32_t idesc = f8_idesc(kBM * G, BN);
+        int i = 0;
+        bool ok = true;
+        for (int t = first; t < tiles && ok; t += step) {
+          for (int k = 0; k < nkb; ++k, ++i) {
+            const int s = i % S, buf = i % NB, use = i / NB;
+            ok = mbar_wait_spin(&full[s], (i / S) & 1, a.max_polls) &&
+                 (use == 0 || mbar_wait_spin(&acc_empty[buf], (use - 1) & 1, a.max_polls));
+            if (!ok) {
+              flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
+              break;
+            }
+            tc_fence_after();
+            const uint64_t ad = sw128_desc(sa + s * L::kA), bd = sw128_desc(sb + s * L::kB);
 #pragma unroll
-        for (int kk = 0; kk < kBK / 32; ++kk)  // 32 bytes of k per MMA along the swizzled rows
-          tc_mma_f8(tmem + buf * BN, ad + 2 * kk, bd + 2 * kk, idesc, kk > 0 ? 1u : 0u);
-        tc_commit(&empty[s]);
-        tc_commit(&acc_full[buf]);
+            for (int kk = 0; kk < kBK / 32; ++kk)  // 32 bytes of k per MMA along the swizzled rows
+              tc_mma_f8<G>(tmem + buf * BN, ad + 2 * kk, bd + 2 * kk, idesc, kk > 0 ? 1u : 0u);
+            tc_commit_group<G>(&acc_full[buf]);
+            tc_commit_group<G>(&empty[s]);
+          }
+        }
+        tc_commit_group<G>(done);
       }
-      tc_commit(done);
+    } else if (warp == 2) {
+      int i = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        const int m0 = tile_m(t), nb0 = tile_n(t) / 128, nb_last = (a.n - 1) / 128;
+        const float *xs[4], *ws[L::kBlocks];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xs[j] = a.xs + (int64_t)min(m0 + lane + 32 * j, a.rows - 1) * a.xs_stride + kb0;
+#pragma unroll
+        for (int b = 0; b < L::kBlocks; ++b) ws[b] = a.ws + (int64_t)min(nb0 + b, nb_last) * a.ws_stride + kb0;
+        for (int k0 = 0; k0 < nkb && ok; k0 += 4) {  // four blocks' loads in flight
+          float x[4][4], w[4][L::kBlocks];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int k = min(k0 + q, nkb - 1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[q][j] = xs[j][k];
+#pragma unroll
+            for (int b = 0; b < L::kBlocks; ++b) w[q][b] = ws[b][k];
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (k0 + q >= nkb || !ok) break;
+            const int slot = i % kScales, use = i / kScales;
+            ok = __all_sync(0xffffffffu,
+                            use == 0 || mbar_wait_spin(&sc_empty[slot], (use - 1) & 1, a.max_polls));
+#pragma unroll
+            for (int b = 0; b < L::kBlocks; ++b)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sc[(slot * L::kBlocks + b) * kBM + lane + 32 * j] = x[q][j] * w[q][b];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sc_full[slot]);
+            ++i;
+          }
+        }
+      }
+      if (!ok) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
     }
   } else {
-    const int lg = warp & 3, part = (warp - 2) >> 2;  // TMEM lanes 32 lg ..; half of the columns
-    const int row = m0 + lg * 32 + lane, col = part * kPart;
-    const float *xs = a.xs + (int64_t)min(row, a.rows - 1) * a.xs_stride + kb0;
-    const float *ws = a.ws + (int64_t)(n0 / 128) * a.ws_stride + kb0;
-    float acc[kPart];
-#pragma unroll
-    for (int j = 0; j < kPart; ++j) acc[j] = 0.f;
-    float scale = xs[0] * ws[0];
-    bool ok = true;
-    for (int i = 0; i < nkb; ++i) {
-      const int buf = i % NB;
-      const float sc = scale;
-      if (i + 1 < nkb) scale = xs[i + 1] * ws[i + 1];
-      if (!mbar_wait_bounded(&acc_full[buf], (i / NB) & 1, a.max_polls)) {
-        ok = false;
-        flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+    if constexpr (G == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+    const int lg = warp & 3, part = (warp - kFirstEpi) >> 2;  // TMEM lanes 32 lg ..; half of the columns
+    const uint32_t tcol = part * CW + ((uint32_t)(lg * 32) << 16);
+    T *stage = reinterpret_cast<T *>(smem + L::kOut) + (warp - kFirstEpi) * 32 * CW;
+    const float *my_sc = sc + part * CW / 128 * kBM + lg * 32 + lane;
+    constexpr int kStretches = CW / ST;
+    static_assert(kStretches % 2 == 0, "two buffers in turn");
+    float2 acc[kStretches][ST / 2];
+    // block i's scales and sums are there
+    auto ready = [&](int i) {
+      const bool ok = mbar_wait_spin(&sc_full[i % kScales], (i / kScales) & 1, a.max_polls) &&
+                      mbar_wait_spin(&acc_full[i % NB], (i / NB) & 1, a.max_polls);
+      const bool all = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      const uint32_t t = tmem + ((uint32_t)(lg * 32) << 16) + buf * BN + col;
+      return all;
+    };
+    int i = 0;
+    bool ok = true;
+    for (int t = first; t < tiles && ok; t += step) {
+      const int row = tile_m(t) + lg * 32 + lane, n0 = tile_n(t) + part * CW;
+      // the sums begin at the bias (where k is split, it is added with the splits)
 #pragma unroll
-      for (int c = 0; c < kPart; c += 32) {
-        uint32_t v[32];
-        tmem_ld<32>(t + c, v);
+      for (int c = 0; c < kStretches; ++c)
 #pragma unroll
-        for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(__uint_as_float(v[j]), sc, acc[c + j]);
+        for (int j = 0; j < ST / 2; ++j) acc[c][j] = make_float2(0.f, 0.f);
+      if (a.bias != nullptr && a.splits == 1) {
+        const T *bias = reinterpret_cast<const T *>(a.bias) + n0;
+#pragma unroll
+        for (int c = 0; c < kStretches; ++c)
+#pragma unroll
+          for (int j = 0; j < ST / 2; ++j) {
+            if (n0 + c * ST + 2 * j < a.n) acc[c][j].x = Elem<T>::to_f32(bias[c * ST + 2 * j]);
+            if (n0 + c * ST + 2 * j + 1 < a.n) acc[c][j].y = Elem<T>::to_f32(bias[c * ST + 2 * j + 1]);
+          }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[buf]);
-    }
-    if (a.splits == 1) {
-      if (ok && row < a.rows)
+      // The loads of one stretch of ST columns are in flight while the last one is added up, and the next
+      // block is waited for meanwhile.
+      uint32_t v[2][ST];
+      ok = ready(i);
+      float scale = my_sc[i % kScales * L::kBlocks * kBM], next = 0.f;
+      if (ok) tmem_ld_async(tmem + i % NB * BN + tcol, v[0]);
+      for (int k = 0; k < nkb && ok; ++k, ++i) {
+        const int buf = i % NB;
 #pragma unroll
-        for (int c = 0; c < kPart; c += 8)
-          if (n0 + col + c < a.n) store_cols<T, 8>(a, row, n0 + col + c, acc + c);
-    } else {
-      // every MMA has read the stages before they are overwritten: this warp saw the last block's results
-      float *tile_s = reinterpret_cast<float *>(smem) + (lg * 32 + lane) * (BN + 4) + col;
+        for (int c = 0; c < kStretches; ++c) {
+          tmem_wait(v[c & 1]);
+          if (c + 1 < kStretches) {
+            tmem_ld_async(tmem + buf * BN + tcol + ST * (c + 1), v[(c + 1) & 1]);
+          } else {
+            // the buffer and the scale have been read
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&sc_empty[i % kScales]);
+              if (G == 1)
+                mbar_arrive(&acc_empty[buf]);
+              else
+                asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(
+                                 map_cluster(smem_u32(&acc_empty[buf]), 0))
+                             : "memory");
+            }
+            if (k + 1 < nkb && ok) tmem_ld_async(tmem + (i + 1) % NB * BN + tcol, v[(c + 1) & 1]);
+          }
+          fma_cols<ST>(acc[c], v[c & 1], scale);
+          if (c == kStretches - 2 && k + 1 < nkb) {
+            ok = ready(i + 1);
+            next = my_sc[(i + 1) % kScales * L::kBlocks * kBM];
+          }
+        }
+        scale = next;
+      }
+      if (!ok) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
+      if (a.splits == 1 && a.tma_out) {
+        // 32 rows by 64 columns at a time, swizzled as TMA reads them, which clips what lies outside
+        const int row0 = row - lane;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last tile's have been read
+        __syncwarp();
 #pragma unroll
-      for (int c = 0; c < kPart; c += 4)
-        if (ok) *reinterpret_cast<float4 *>(tile_s + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+        for (int c = 0; c < CW / 8; ++c) {
+          T o[8];
+          round_cols<T, 8>(&acc[8 * c / ST][8 * c % ST / 2].x, o);
+          uint4 *dst = reinterpret_cast<uint4 *>(stage + c / 8 * (32 * 64) + lane * 64);
+          dst[(c % 8) ^ (lane & 7)] = pack_8(o);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0 && ok && row0 < a.rows) {
+#pragma unroll
+          for (int c = 0; c < CW / 64; ++c)
+            if (n0 + 64 * c < a.n)
+              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                               reinterpret_cast<uint64_t>(&to)),
+                           "r"(n0 + 64 * c), "r"(row0), "r"(smem_u32(stage + c * (32 * 64)))
+                           : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+      } else if (a.splits == 1) {
+        if (ok && row < a.rows) {
+#pragma unroll
+          for (int c = 0; c < CW / 8; ++c)
+            if (n0 + 8 * c < a.n) store_cols<T, 8>(a, row, n0 + 8 * c, &acc[8 * c / ST][8 * c % ST / 2].x);
+        }
+      } else {
+        // every MMA has read the stages before they are overwritten: this warp saw the last block's results
+        float *tile_s = reinterpret_cast<float *>(smem) + (lg * 32 + lane) * (BN + 4) + part * CW;
+        if (ok) {
+#pragma unroll
+          for (int c = 0; c < CW / 4; ++c)
+            *reinterpret_cast<float4 *>(tile_s + 4 * c) =
+                make_float4(acc[4 * c / ST][4 * c % ST / 2].x, acc[4 * c / ST][4 * c % ST / 2].y,
+                            acc[4 * c / ST][4 * c % ST / 2 + 1].x, acc[4 * c / ST][4 * c % ST / 2 + 1].y);
+        }
+      }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
   __syncthreads();
-  if (a.splits > 1) {
+  if (G == 1 && a.splits > 1) {  // one tile per cluster
     cluster_sync();
+    const int m0 = tile_m(first), n0 = tile_n(first);
     const uint32_t base = smem_u32(smem);
     constexpr int kC4 = BN / 4;
-    const int my_rows = (kBM - split + a.splits - 1) / a.splits;
+    const int my_rows = (min(kBM, a.rows - m0) - split + a.splits - 1) / a.splits;
     for (int it = threadIdx.x; it < my_rows * kC4; it += kThreads) {
       const int r = split + (it / kC4) * a.splits, c4 = it % kC4;
-      if (m0 + r >= a.rows || n0 + 4 * c4 >= a.n) continue;
+      if (n0 + 4 * c4 >= a.n) continue;
       const uint32_t off = (uint32_t)((r * (BN + 4) + 4 * c4) * sizeof(float));
       float v[4] = {0.f, 0.f, 0.f, 0.f};
       for (int sp = 0; sp < a.splits; ++sp) {
@@ -251,62 +505,101 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
         v[2] += p.z;
         v[3] += p.w;
       }
+      if (a.bias != nullptr) {
+        const T *bias = reinterpret_cast<const T *>(a.bias) + n0 + 4 * c4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n0 + 4 * c4 + j < a.n) v[j] += Elem<T>::to_f32(bias[j]);
+      }
       store_cols<T, 4>(a, m0 + r, n0 + 4 * c4, v);
     }
     cluster_sync();
   }
   if (warp == 1) {
-    if (lane == 0 && !mbar_wait_bounded(done, 0, a.max_polls)) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
+    if (lane == 0 && !mbar_wait_spin(done, 0, a.max_polls)) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
     __syncwarp();
+  }
+  if (G == 2) cluster_sync();  // no MMA of the pair is in flight, nothing arrives at a CTA that has gone
+  if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kCols) : "memory");
+    if constexpr (G == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
 }
 
-// 2-D map of a row-major [rows, k] byte matrix, boxes of 128 (k) by box_rows
-// rows, 128-byte swizzle, zero fill outside the matrix.
-int encode_bytes(CUtensorMap *map, const void *base, int64_t k, int64_t rows, int64_t row_stride,
-                 uint32_t box_rows) {
+// 2-D map of a row-major [rows, cols] matrix of `type`, boxes of 128 bytes of a
+// row by box_rows rows, 128-byte swizzle; loads read zeros outside the matrix.
+int encode_rows(CUtensorMap *map, CUtensorMapDataType type, int size, const void *base, int64_t cols, int64_t rows,
+                int64_t row_stride, uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) {
     set_error_detail("pkv_linear_fp8: cuTensorMapEncodeTiled is not available from the driver");
     return PKV_ERR_TENSOR_MAP;
   }
-  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)row_stride};
-  const cuuint32_t box[2] = {(cuuint32_t)kBK, box_rows}, elem[2] = {1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, elem,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(row_stride * size)};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / size), box_rows}, elem[2] = {1, 1};
+  const CUresult r = fn(map, type, 2, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error_detail("pkv_linear_fp8: cuTensorMapEncodeTiled failed (%d) for a [%lld, %lld] matrix", (int)r,
-                     (long long)rows, (long long)k);
+                     (long long)rows, (long long)cols);
     return PKV_ERR_TENSOR_MAP;
   }
   return PKV_OK;
 }
 
-template <typename T, int BN, int S>
-int fp8_launch(const CUtensorMap &tx, const CUtensorMap &tw, const Fp8Args &a, cudaStream_t st) {
-  using L = Smem<BN, S>;
+template <typename T, int BN, int S, int G>
+int fp8_launch(const void *x, const void *w, int64_t k, int64_t x_stride, int64_t w_stride, Fp8Args a,
+               cudaStream_t st) {
+  using L = Smem<BN, S, G>;
   static_assert(L::kBytes <= 227 * 1024, "shared memory");
-  static_assert(kBM * (BN + 4) * sizeof(float) <= L::kFull, "the split tile fits the ring");
-  auto kern = linear_fp8_kernel<T, BN, S>;
+  static_assert(G == 2 || kBM * (BN + 4) * sizeof(float) <= L::kSc, "the split tile fits the ring");
+  CUtensorMap tx, tw, to;
+  int rc = encode_rows(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, k, a.rows, x_stride, kBM);
+  if (rc == PKV_OK) rc = encode_rows(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, k, a.n, w_stride, BN / G);
+  to = tx;
+  a.tma_out = aligned_to(a.out, 16) && a.out_stride % 8 == 0;
+  if (rc == PKV_OK && a.tma_out)
+    rc = encode_rows(&to, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, a.out, a.n, a.rows, a.out_stride, 32);
+  if (rc != PKV_OK) return rc;
+  auto kern = linear_fp8_kernel<T, BN, S, G>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes) != cudaSuccess)
     return check_launch("cudaFuncSetAttribute(linear_fp8)");
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+  const int cluster = G == 2 ? 2 : a.splits;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits));
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(tiles * cluster, lin_sms() / cluster * cluster));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = L::kBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)a.splits;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = a.splits > 1 ? 1 : 0;
-  (void)cudaLaunchKernelEx(&cfg, kern, tx, tw, a);
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  (void)cudaLaunchKernelEx(&cfg, kern, tx, tw, to, a);
   return check_launch("linear_fp8_kernel");
+}
+
+template <typename T>
+int fp8_dispatch(const void *x, const void *w, int64_t k, int64_t x_stride, int64_t w_stride, Fp8Args a,
+                 cudaStream_t st) {
+  const int sms = lin_sms();
+  auto tiles = [&](int bm, int bn) {
+    a.tiles_m = (a.rows - 1) / bm + 1;
+    a.tiles_n = (a.n - 1) / bn + 1;
+    return (int64_t)a.tiles_m * a.tiles_n;
+  };
+  a.splits = 1;
+  if (a.rows > kBM && tiles(256, 256) >= sms / 2) return fp8_launch<T, 256, 4, 2>(x, w, k, x_stride, w_stride, a, st);
+  const int64_t t = tiles(128, 128);
+  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)a.kblocks, (int64_t)kMaxSplits, sms / t}));
+  return fp8_launch<T, 128, 5, 1>(x, w, k, x_stride, w_stride, a, st);
 }
 
 }  // namespace
@@ -351,22 +644,12 @@ extern "C" int pkv_linear_fp8(const void *x, const float *x_scale, const void *w
   a.rows = rows;
   a.n = n;
   a.kblocks = kblocks;
-  constexpr int BN = 128;
-  a.tiles_m = (rows - 1) / kBM + 1;
-  a.tiles_n = (n - 1) / BN + 1;
-  a.splits = (int)std::max<int64_t>(
-      1, std::min<int64_t>({(int64_t)kblocks, (int64_t)kMaxSplits, lin_sms() / ((int64_t)a.tiles_m * a.tiles_n)}));
   a.max_polls = kMaxPolls;
-  if ((int64_t)a.tiles_m * a.tiles_n * a.splits > INT32_MAX) {
+  if (((int64_t)(rows - 1) / kBM + 1) * ((n - 1) / 128 + 1) > INT32_MAX / 2) {
     set_error_detail("pkv_linear_fp8: too many tiles");
     return PKV_ERR_UNSUPPORTED;
   }
-  CUtensorMap tx, tw;
-  int rc = encode_bytes(&tx, x, k, rows, x_stride, kBM);
-  if (rc) return rc;
-  rc = encode_bytes(&tw, w, k, n, w_stride, BN);
-  if (rc) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return out_dtype == PKV_DTYPE_BF16 ? fp8_launch<__nv_bfloat16, BN, 6>(tx, tw, a, st)
-                                     : fp8_launch<__half, BN, 6>(tx, tw, a, st);
+  return out_dtype == PKV_DTYPE_BF16 ? fp8_dispatch<__nv_bfloat16>(x, w, k, x_stride, w_stride, a, st)
+                                     : fp8_dispatch<__half>(x, w, k, x_stride, w_stride, a, st);
 }
