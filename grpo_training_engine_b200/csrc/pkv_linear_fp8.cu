@@ -18,7 +18,7 @@
 //   warp 1             : TMEM allocation; one thread (of the pair's first CTA)
 //                        issues the 4 MMAs (M 128 G, N BN, K 32) of each block
 //   warp 2             : the products of the two scales for each row and block,
-//                        into a ring of their own: straight from global memory
+//                        beside the TMEM buffers: straight from global memory
 //                        every epilogue thread's load would be a line of its own
 //   warps 4-11         : two warps per 32-lane TMEM group, half of the columns
 //                        each: accumulate block by block, then store through
@@ -46,7 +46,6 @@ constexpr int kFirstEpi = 4;         // first epilogue warp: its warpgroup is al
 constexpr int kEpiWarps = 8, kThreads = 32 * (kFirstEpi + kEpiWarps);
 // registers per thread: 384 threads start with 168 each, 64512 in all = 128 x 72 + 256 x 216
 constexpr int kRegsOther = 72, kRegsEpi = 216;
-constexpr int kScales = 8;           // k blocks whose scales are ready ahead
 
 struct Fp8Args {
   const float *xs, *ws;  // scales: rows of x, blocks of W
@@ -55,6 +54,7 @@ struct Fp8Args {
   int32_t *status;
   int64_t xs_stride, ws_stride, out_stride;
   int32_t rows, n, kblocks, tiles_m, tiles_n, splits;
+  int32_t x_rows;   // rows of x that a tile loads (the MMA's others hold what they hold: their sums go nowhere)
   int32_t tma_out;  // out can be stored by TMA: 16-byte aligned base and rows
   uint32_t max_polls;
 };
@@ -122,7 +122,7 @@ __host__ __device__ constexpr uint32_t f8_idesc(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// 32 columns of this thread's TMEM lane; the values are there after tmem_wait.
+// 32 or 16 columns of this thread's TMEM lane; the values are there after tmem_wait.
 __device__ __forceinline__ void tmem_ld_async(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -133,7 +133,21 @@ __device__ __forceinline__ void tmem_ld_async(uint32_t taddr, uint32_t (&v)[32])
         "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld_async(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
 // Waits for this thread's loads; passing the registers through keeps their uses behind it.
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
@@ -159,22 +173,23 @@ __device__ __forceinline__ void fma_cols(float2 (&acc)[N / 2], const uint32_t (&
 __device__ __forceinline__ uint32_t bits16(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 __device__ __forceinline__ uint32_t bits16(__half v) { return __half_as_ushort(v); }
 
-template <int BN, int S, int G>
+// P CTAs share an SM.
+template <int BN, int S, int G, int P>
 struct Smem {
   static constexpr int kA = kBM * kBK, kB = BN / G * kBK;  // one stage of x and of W, bytes
-  static constexpr int kBufs = 512 / BN;                   // TMEM buffers of BN fp32 columns: all 512 columns
+  static constexpr int kCols = 512 / P;                    // TMEM columns
+  static constexpr int kBufs = kCols / BN;                 // TMEM buffers of BN fp32 columns
   static constexpr int kCW = BN / 2;                       // columns of an epilogue warp
   static constexpr int kBlocks = (BN + 127) / 128;         // blocks of W's scales across a tile
   static constexpr size_t kW = (size_t)S * kA;
   static constexpr size_t kOut = kW + (size_t)S * kB;      // 32 rows x kCW 16-bit results of each epilogue warp
-  static constexpr size_t kSc = kOut + (size_t)kEpiWarps * 32 * kCW * 2;  // [kScales][kBlocks][kBM] fp32
-  static constexpr size_t kFull = kSc + 4 * kScales * kBlocks * kBM;
+  static constexpr bool kStage = P == 1;                   // (two CTAs on an SM hide each other's direct stores)
+  static constexpr size_t kSc = kOut + (kStage ? kEpiWarps * 32 * kCW * 2 : 0);  // [kBufs][kBlocks][kBM] fp32
+  static constexpr size_t kFull = kSc + 4 * kBufs * kBlocks * kBM;
   static constexpr size_t kEmpty = kFull + 8 * S;
   static constexpr size_t kAccFull = kEmpty + 8 * S;
   static constexpr size_t kAccEmpty = kAccFull + 8 * kBufs;
-  static constexpr size_t kScFull = kAccEmpty + 8 * kBufs;
-  static constexpr size_t kScEmpty = kScFull + 8 * kScales;
-  static constexpr size_t kDone = kScEmpty + 8 * kScales;
+  static constexpr size_t kDone = kAccEmpty + 8 * kBufs;
   static constexpr size_t kTmem = kDone + 8;
   static constexpr size_t kBytes = kTmem + 8 + 1024;  // + alignment slack
 };
@@ -208,12 +223,12 @@ __device__ __forceinline__ void store_cols(const Fp8Args &a, int row, int col, c
     if (col + j < a.n) out[j] = o[j];
 }
 
-template <typename T, int BN, int S, int G>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int BN, int S, int G, int P>
+__global__ void __launch_bounds__(kThreads, P)
 linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
                   const __grid_constant__ CUtensorMap to, Fp8Args a) {
-  using L = Smem<BN, S, G>;
-  constexpr int NB = L::kBufs, CW = L::kCW, ST = 32;
+  using L = Smem<BN, S, G, P>;
+  constexpr int NB = L::kBufs, CW = L::kCW, ST = CW >= 64 ? 32 : 16;
   extern __shared__ uint8_t raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   uint8_t *sa = smem, *sb = smem + L::kW;
@@ -222,8 +237,6 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
   uint64_t *acc_full = reinterpret_cast<uint64_t *>(smem + L::kAccFull);
   uint64_t *acc_empty = reinterpret_cast<uint64_t *>(smem + L::kAccEmpty);
   uint64_t *done = reinterpret_cast<uint64_t *>(smem + L::kDone);
-  uint64_t *sc_full = reinterpret_cast<uint64_t *>(smem + L::kScFull);
-  uint64_t *sc_empty = reinterpret_cast<uint64_t *>(smem + L::kScEmpty);
   float *sc = reinterpret_cast<float *>(smem + L::kSc);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::kTmem);
 
@@ -242,12 +255,8 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < NB; ++s) {
-      mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], kEpiWarps * G);
-    }
-    for (int s = 0; s < kScales; ++s) {
-      mbar_init(&sc_full[s], 1);
-      mbar_init(&sc_empty[s], kEpiWarps);
+      mbar_init(&acc_full[s], 2);  // the MMAs, the scales
+      mbar_init(&acc_empty[s], rank == 0 ? kEpiWarps * G : kEpiWarps);
     }
     mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -258,12 +267,12 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
   if (warp == 1) {
     if constexpr (G == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                   "r"(512)
+                   "r"(L::kCols)
                    : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                   "r"(512)
+                   "r"(L::kCols)
                    : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
@@ -293,7 +302,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
             }
             uint32_t bar = smem_u32(&full[s]);
             if (G == 2) bar = map_cluster(bar, 0);
-            if (rank == 0) mbar_expect_tx(&full[s], G * (L::kA + L::kB));
+            if (rank == 0) mbar_expect_tx(&full[s], G * (a.x_rows * kBK + L::kB));
             tma_load_group<G>(sa + s * L::kA, &tx, (kb0 + k) * kBK, m0, bar);
             tma_load_group<G>(sb + s * L::kB, &tw, (kb0 + k) * kBK, n0, bar);
             ++issued;
@@ -331,40 +340,45 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
         tc_commit_group<G>(done);
       }
     } else if (warp == 2) {
-      int i = 0;
-      bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
+      // four blocks at a time, the next four's loads in flight while these are handed out
+      struct Group {
+        float x[4][4], w[4][L::kBlocks];  // [block][32 rows], [block][128 columns]
+      };
+      auto load = [&](int t, int k0, Group &g) {
         const int m0 = tile_m(t), nb0 = tile_n(t) / 128, nb_last = (a.n - 1) / 128;
-        const float *xs[4], *ws[L::kBlocks];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) xs[j] = a.xs + (int64_t)min(m0 + lane + 32 * j, a.rows - 1) * a.xs_stride + kb0;
+        for (int q = 0; q < 4; ++q) {
+          const int k = kb0 + min(k0 + q, nkb - 1);
 #pragma unroll
-        for (int b = 0; b < L::kBlocks; ++b) ws[b] = a.ws + (int64_t)min(nb0 + b, nb_last) * a.ws_stride + kb0;
-        for (int k0 = 0; k0 < nkb && ok; k0 += 4) {  // four blocks' loads in flight
-          float x[4][4], w[4][L::kBlocks];
+          for (int j = 0; j < 4; ++j)
+            g.x[q][j] = m0 + 32 * j < a.rows ? a.xs[min(m0 + lane + 32 * j, a.rows - 1) * a.xs_stride + k] : 0.f;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int k = min(k0 + q, nkb - 1);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[q][j] = xs[j][k];
-#pragma unroll
-            for (int b = 0; b < L::kBlocks; ++b) w[q][b] = ws[b][k];
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (k0 + q >= nkb || !ok) break;
-            const int slot = i % kScales, use = i / kScales;
-            ok = __all_sync(0xffffffffu,
-                            use == 0 || mbar_wait_spin(&sc_empty[slot], (use - 1) & 1, a.max_polls));
-#pragma unroll
-            for (int b = 0; b < L::kBlocks; ++b)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) sc[(slot * L::kBlocks + b) * kBM + lane + 32 * j] = x[q][j] * w[q][b];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sc_full[slot]);
-            ++i;
-          }
+          for (int b = 0; b < L::kBlocks; ++b) g.w[q][b] = a.ws[min(nb0 + b, nb_last) * a.ws_stride + k];
         }
+      };
+      int i = 0, t = first, k0 = 0;
+      bool ok = true;
+      Group now, next;
+      if (t < tiles) load(t, 0, now);
+      while (t < tiles && ok) {
+        const int kn = k0 + 4 < nkb ? k0 + 4 : 0, tn = kn > 0 ? t : t + step;
+        if (tn < tiles) load(tn, kn, next);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (k0 + q >= nkb || !ok) break;
+          const int slot = i % NB, use = i / NB;
+          ok = __all_sync(0xffffffffu, use == 0 || mbar_wait_spin(&acc_empty[slot], (use - 1) & 1, a.max_polls));
+#pragma unroll
+          for (int b = 0; b < L::kBlocks; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[(slot * L::kBlocks + b) * kBM + lane + 32 * j] = now.x[q][j] * now.w[q][b];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_full[slot]);
+          ++i;
+        }
+        now = next;
+        t = tn;
+        k0 = kn;
       }
       if (!ok) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
     }
@@ -377,10 +391,9 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
     constexpr int kStretches = CW / ST;
     static_assert(kStretches % 2 == 0, "two buffers in turn");
     float2 acc[kStretches][ST / 2];
-    // block i's scales and sums are there
+    // block i's sums and scales are there
     auto ready = [&](int i) {
-      const bool ok = mbar_wait_spin(&sc_full[i % kScales], (i / kScales) & 1, a.max_polls) &&
-                      mbar_wait_spin(&acc_full[i % NB], (i / NB) & 1, a.max_polls);
+      const bool ok = mbar_wait_spin(&acc_full[i % NB], (i / NB) & 1, a.max_polls);
       const bool all = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       return all;
@@ -408,7 +421,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
       // block is waited for meanwhile.
       uint32_t v[2][ST];
       ok = ready(i);
-      float scale = my_sc[i % kScales * L::kBlocks * kBM], next = 0.f;
+      float scale = my_sc[i % NB * L::kBlocks * kBM], next = 0.f;
       if (ok) tmem_ld_async(tmem + i % NB * BN + tcol, v[0]);
       for (int k = 0; k < nkb && ok; ++k, ++i) {
         const int buf = i % NB;
@@ -422,26 +435,25 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-              mbar_arrive(&sc_empty[i % kScales]);
-              if (G == 1)
-                mbar_arrive(&acc_empty[buf]);
-              else
+              mbar_arrive(&acc_empty[buf]);
+              if (rank == 1)  // for the MMAs, which the pair's first CTA issues
                 asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(
                                  map_cluster(smem_u32(&acc_empty[buf]), 0))
                              : "memory");
             }
+            __syncwarp();  // (the loads are a whole warp's)
             if (k + 1 < nkb && ok) tmem_ld_async(tmem + (i + 1) % NB * BN + tcol, v[(c + 1) & 1]);
           }
           fma_cols<ST>(acc[c], v[c & 1], scale);
           if (c == kStretches - 2 && k + 1 < nkb) {
             ok = ready(i + 1);
-            next = my_sc[(i + 1) % kScales * L::kBlocks * kBM];
+            next = my_sc[(i + 1) % NB * L::kBlocks * kBM];
           }
         }
         scale = next;
       }
       if (!ok) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
-      if (a.splits == 1 && a.tma_out) {
+      if (L::kStage && a.splits == 1 && a.tma_out) {
         // 32 rows by 64 columns at a time, swizzled as TMA reads them, which clips what lies outside
         const int row0 = row - lane;
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last tile's have been read
@@ -523,9 +535,9 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
   if (warp == 1) {
     tc_fence_after();
     if constexpr (G == 1)
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kCols) : "memory");
     else
-      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kCols) : "memory");
   }
 }
 
@@ -551,27 +563,28 @@ int encode_rows(CUtensorMap *map, CUtensorMapDataType type, int size, const void
   return PKV_OK;
 }
 
-template <typename T, int BN, int S, int G>
+template <typename T, int BN, int S, int G, int P>
 int fp8_launch(const void *x, const void *w, int64_t k, int64_t x_stride, int64_t w_stride, Fp8Args a,
                cudaStream_t st) {
-  using L = Smem<BN, S, G>;
+  using L = Smem<BN, S, G, P>;
   static_assert(L::kBytes <= 227 * 1024, "shared memory");
   static_assert(G == 2 || kBM * (BN + 4) * sizeof(float) <= L::kSc, "the split tile fits the ring");
+  a.x_rows = std::min(kBM, (a.rows + 7) / 8 * 8);
   CUtensorMap tx, tw, to;
-  int rc = encode_rows(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, k, a.rows, x_stride, kBM);
+  int rc = encode_rows(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, k, a.rows, x_stride, a.x_rows);
   if (rc == PKV_OK) rc = encode_rows(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, k, a.n, w_stride, BN / G);
   to = tx;
-  a.tma_out = aligned_to(a.out, 16) && a.out_stride % 8 == 0;
+  a.tma_out = L::kStage && aligned_to(a.out, 16) && a.out_stride % 8 == 0;
   if (rc == PKV_OK && a.tma_out)
     rc = encode_rows(&to, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, a.out, a.n, a.rows, a.out_stride, 32);
   if (rc != PKV_OK) return rc;
-  auto kern = linear_fp8_kernel<T, BN, S, G>;
+  auto kern = linear_fp8_kernel<T, BN, S, G, P>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes) != cudaSuccess)
     return check_launch("cudaFuncSetAttribute(linear_fp8)");
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
   const int cluster = G == 2 ? 2 : a.splits;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min<int64_t>(tiles * cluster, lin_sms() / cluster * cluster));
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(tiles * cluster, lin_sms() * P / cluster * cluster));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = L::kBytes;
   cfg.stream = st;
@@ -596,10 +609,11 @@ int fp8_dispatch(const void *x, const void *w, int64_t k, int64_t x_stride, int6
     return (int64_t)a.tiles_m * a.tiles_n;
   };
   a.splits = 1;
-  if (a.rows > kBM && tiles(256, 256) >= sms / 2) return fp8_launch<T, 256, 4, 2>(x, w, k, x_stride, w_stride, a, st);
-  const int64_t t = tiles(128, 128);
-  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)a.kblocks, (int64_t)kMaxSplits, sms / t}));
-  return fp8_launch<T, 128, 5, 1>(x, w, k, x_stride, w_stride, a, st);
+  if (a.rows > kBM && tiles(256, 256) >= sms / 2)
+    return fp8_launch<T, 256, 4, 2, 1>(x, w, k, x_stride, w_stride, a, st);
+  const int64_t t = tiles(128, 64);
+  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)a.kblocks, (int64_t)kMaxSplits, 2 * sms / t}));
+  return fp8_launch<T, 64, 4, 1, 2>(x, w, k, x_stride, w_stride, a, st);
 }
 
 }  // namespace
