@@ -23,7 +23,7 @@ INCLUDE = REPO_DIR / "include"
 LIB_PATH = PKG_DIR / "libpkv.so"
 
 SOURCES = ["pkv_copy.cu", "pkv_decode.cu", "pkv_noalloc.cu", "pkv_sample.cu", "pkv_glue.cu", "pkv_linear.cu",
-           "pkv_fp8.cu", "pkv_linear_fp8.cu", "pkv_loss.cu"]
+           "pkv_fp8.cu", "pkv_linear_fp8.cu", "pkv_linear_fp8_rows.cu", "pkv_loss.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -38,6 +38,13 @@
 #include "pkv_types.cuh"
 
 namespace pkv {
+
+// pkv_linear_fp8_rows.cu: the product for a few rows
+bool linear_fp8_rows_fits(int32_t rows, int32_t n, int32_t k);
+int linear_fp8_rows(const void *x, const float *x_scale, const void *w, const float *w_scale, const void *bias,
+                    void *out, int32_t rows, int32_t n, int32_t k, int64_t x_stride, int64_t xs_stride,
+                    int64_t w_stride, int64_t ws_stride, int64_t out_stride, int32_t out_dtype, void *stream);
+
 namespace {
 
 constexpr int kBM = 128, kBK = 128;  // tile rows; k values of a block, the span of one scale
@@ -183,7 +190,7 @@ struct Smem {
   static constexpr int kBlocks = (BN + 127) / 128;         // blocks of W's scales across a tile
   static constexpr size_t kW = (size_t)S * kA;
   static constexpr size_t kOut = kW + (size_t)S * kB;      // 32 rows x kCW 16-bit results of each epilogue warp
-  static constexpr bool kStage = P == 1;                   // (two CTAs on an SM hide each other's direct stores)
+  static constexpr bool kStage = G == 2;                   // (few rows: direct stores)
   static constexpr size_t kSc = kOut + (kStage ? kEpiWarps * 32 * kCW * 2 : 0);  // [kBufs][kBlocks][kBM] fp32
   static constexpr size_t kFull = kSc + 4 * kBufs * kBlocks * kBM;
   static constexpr size_t kEmpty = kFull + 8 * S;
@@ -229,6 +236,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
                   const __grid_constant__ CUtensorMap to, Fp8Args a) {
   using L = Smem<BN, S, G, P>;
   constexpr int NB = L::kBufs, CW = L::kCW, ST = CW >= 64 ? 32 : 16;
+  constexpr bool kSplitRegs = CW == 128;  // 128 sums per epilogue thread
   extern __shared__ uint8_t raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   uint8_t *sa = smem, *sb = smem + L::kW;
@@ -286,7 +294,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
   auto tile_n = [&](int t) { return (t / a.tiles_m) * BN; };
 
   if (warp < kFirstEpi) {
-    if constexpr (G == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if constexpr (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == 0) {
       if (lane == 0) {
         int i = 0, issued = 0;
@@ -383,7 +391,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
       if (!ok) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
     }
   } else {
-    if constexpr (G == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+    if constexpr (kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     const int lg = warp & 3, part = (warp - kFirstEpi) >> 2;  // TMEM lanes 32 lg ..; half of the columns
     const uint32_t tcol = part * CW + ((uint32_t)(lg * 32) << 16);
     T *stage = reinterpret_cast<T *>(smem + L::kOut) + (warp - kFirstEpi) * 32 * CW;
@@ -609,8 +617,14 @@ int fp8_dispatch(const void *x, const void *w, int64_t k, int64_t x_stride, int6
     return (int64_t)a.tiles_m * a.tiles_n;
   };
   a.splits = 1;
+  // Many rows: pairs, whose 256 x 256 tiles read least from L2 for what they multiply (4096 x 18944 x 3584: 336 us
+  // against 426 with 128 x 128 tiles, which stop at 10 TB/s out of L2).
   if (a.rows > kBM && tiles(256, 256) >= sms / 2)
     return fp8_launch<T, 256, 4, 2, 1>(x, w, k, x_stride, w_stride, a, st);
+  // Wide matrices: an MMA of 256 columns takes little longer than one of 64 (151,936 columns by 37 rows: 54 us
+  // against 67).
+  if (tiles(128, 256) >= 2 * sms) return fp8_launch<T, 256, 4, 1, 1>(x, w, k, x_stride, w_stride, a, st);
+  // The rest: narrow tiles, two CTAs on an SM, k split until they fill the machine.
   const int64_t t = tiles(128, 64);
   a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)a.kblocks, (int64_t)kMaxSplits, 2 * sms / t}));
   return fp8_launch<T, 64, 4, 1, 2>(x, w, k, x_stride, w_stride, a, st);
@@ -646,6 +660,9 @@ extern "C" int pkv_linear_fp8(const void *x, const float *x_scale, const void *w
                      (long long)x_stride, (long long)w_stride);
     return PKV_ERR_ALIGNMENT;
   }
+  if (linear_fp8_rows_fits(rows, n, k))
+    return linear_fp8_rows(x, x_scale, w, w_scale, bias, out, rows, n, k, x_stride, xs_stride, w_stride, ws_stride,
+                           out_stride, out_dtype, stream);
   Fp8Args a{};
   a.xs = x_scale;
   a.ws = w_scale;
