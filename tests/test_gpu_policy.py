@@ -367,3 +367,11 @@ def test_policy_loss_empty_and_other_stream():
         got = ops.policy_loss(logits, tokens, old, adv, mask, ref_logprobs=ref, kl_coef=0.1)
     st.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_no_second_derivatives():
+    logits, tokens, old, adv, mask, _ = _batch(2, 3, 20, torch.float32, 6)
+    leaf = logits.requires_grad_()
+    for loss in (ops.policy_loss(leaf, tokens, old, adv, mask).loss, ops.token_logprobs(leaf, tokens).sum()):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(loss, leaf, create_graph=True)
