@@ -832,6 +832,10 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
         const int held = min(sl.hi, a.hold);
         for (int k = 0; k < K; ++k) {
           if (it > 0) ok = mbar_wait_bounded(&sh.empty[k], (it - 1) & 1) && ok;
+          if (k == K / 2 && sl.hi > held)  // what is not held, on its way to L2 before the consumers stream it
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(sl.vecs() + held),
+                         "r"((sl.hi - held) * 16)
+                         : "memory");
           const int c0 = chunk(held, k), bytes = (chunk(held, k + 1) - c0) * 16;
           mbar_expect(&sh.full[k], bytes);
           if (bytes > 0)
@@ -892,6 +896,9 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
       const int held = min(sl.hi, a.hold), held_n = min(sn.hi, a.hold);
       T *out = grad + r * (int64_t)a.vocab;
       st = Soft();
+      // what is not held first: it is the longest since it was read, and the chunks' refills are then in flight
+      // until the end
+      grad_range<T, false, NT>(sl, g, out, sl.vecs() + held, held, sl.hi, tid);
       for (int k = 0; k < K; ++k) {
         const int c0 = chunk(held, k), c1 = chunk(held, k + 1);
         grad_range<T, false, NT>(sl, g, out, hv + c0, c0, c1, tid);
@@ -899,7 +906,6 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
         if (lane == 0) mbar_arrive(&sh.empty[k]);
         if (more && k > 0) sum_chunk(st, held_n, k - 1, it + 1);
       }
-      grad_range<T, false, NT>(sl, g, out, sl.vecs() + held, held, sl.hi, tid);
       grad_edge<T, false>(sl, g, out, tid);
       if (more) {
         sum_rest(st, sn, held_n);
@@ -986,10 +992,10 @@ int launch_grad(const T *logits, Rows rows, T *grad, const PolicyArgs &a, void *
   if (bytes <= 32 * 16 * 16) return launch_row<T, 32, 16, 4, 4>(logits, rows, grad, a, stream);
   if (bytes <= 128 * 16 * 16) return launch_row<T, 128, 16, 1, 4>(logits, rows, grad, a, stream);
   if (bytes <= 256 * 16 * 16) return launch_row<T, 256, 16, 1, 2>(logits, rows, grad, a, stream);
-  // two blocks on an SM hold 96 KB each: 304 KB rows take 535 us for 4096 in one block and 568 in two, 100 KB rows
-  // 254 and 182 us for 4096, 200 KB rows 185 and 174 us for 2048
+  // Two blocks on an SM, 96 KB of a row each, or one with 168 KB: rows of 100 KB take 176 us for 4096 in two and 254
+  // in one, of 200 KB 167 us for 2048 in two and 175 in one, of 304 KB 568 us for 4096 in two and 481 in one.
   if (bytes <= 200 * 1024) return launch_held<T, 384, 4, 2>(logits, rows, grad, a, stream);
-  return launch_held<T, 768, 4, 1>(logits, rows, grad, a, stream);
+  return launch_held<T, 896, 3, 1>(logits, rows, grad, a, stream);
 }
 
 bool bad_logits(const char *fn, const void *logits, int32_t dtype, int64_t rows, int32_t vocab, int32_t inner,
