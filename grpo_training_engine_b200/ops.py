@@ -55,15 +55,15 @@ def _dtype_code(t: torch.Tensor, what: str) -> int:
 
 
 def _require_cuda(*tensors: Optional[torch.Tensor]) -> torch.device:
-    dev = None
+    dev, index = None, -1
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
             raise ValueError("inputs and caches must be on CUDA device.")
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
+            dev, index = t.device, t.get_device()
+        elif t.get_device() != index:
             raise ValueError(f"all tensors must be on one device, got {dev} and {t.device}.")
     assert dev is not None
     return dev
@@ -717,6 +717,18 @@ def sample_top_p(
 # ---------------------------------------------------------------------------
 # 8-bit activations and weights
 # ---------------------------------------------------------------------------
+def _call(dev: torch.device, name: str, *args) -> None:
+    """One entry point of libpkv.so on `dev`'s current stream (the last argument)."""
+    fn = getattr(_lib.load(), name)
+    if dev.index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc < 0:
+        raise _lib.PkvError(name, rc, _lib.last_detail())
+
+
 FP8_GROUP = 128  # values that share a scale
 
 
@@ -763,14 +775,9 @@ def add_rmsnorm_fp8(
     q = _fp8_rows(rows, hidden, dev)
     scales = _empty2(rows, _groups(hidden), torch.float32, dev)
     total = _empty2(rows, hidden, x.dtype, dev) if residual is not None else None
-    with _device_ctx(dev):
-        _lib.check(
-            "pkv_add_rmsnorm_fp8",
-            _lib.load().pkv_add_rmsnorm_fp8(
-                x.data_ptr(), _lib.ptr(residual), weight.data_ptr(), _lib.ptr(total), q.data_ptr(),
-                scales.data_ptr(), rows, hidden, x.stride(0), residual.stride(0) if residual is not None else 0,
-                hidden, q.stride(0), scales.stride(0), eps, code, _stream(dev)),
-        )
+    _call(dev, "pkv_add_rmsnorm_fp8", x.data_ptr(), _lib.ptr(residual), weight.data_ptr(), _lib.ptr(total),
+          q.data_ptr(), scales.data_ptr(), rows, hidden, x.stride(0),
+          residual.stride(0) if residual is not None else 0, hidden, q.stride(0), scales.stride(0), eps, code)
     return q, scales, total
 
 
@@ -782,12 +789,8 @@ def _quantize_fp8(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch
     rows, cols = x.shape
     q = _fp8_rows(rows, cols, dev)
     scales = torch.empty(((rows + block_rows - 1) // block_rows, _groups(cols)), dtype=torch.float32, device=dev)
-    with _device_ctx(dev):
-        _lib.check(
-            "pkv_quantize_fp8",
-            _lib.load().pkv_quantize_fp8(x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, cols, block_rows,
-                                         x.stride(0), q.stride(0), scales.stride(0), code, _stream(dev)),
-        )
+    _call(dev, "pkv_quantize_fp8", x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, cols, block_rows,
+          x.stride(0), q.stride(0), scales.stride(0), code)
     return q, scales
 
 
@@ -849,15 +852,10 @@ def linear_fp8(
         out = _empty2(rows, n, out_dtype, dev)
     elif out.shape != (rows, n) or out.stride(1) != 1 or (rows > 1 and out.stride(0) < n):
         raise ValueError(f"out must be a [rows, {n}] tensor with contiguous rows that do not overlap.")
-    with _device_ctx(dev):
-        _lib.check(
-            "pkv_linear_fp8",
-            _lib.load().pkv_linear_fp8(
-                x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(), _lib.ptr(bias),
-                out.data_ptr(), rows, n, k, x_stride, x_scale.stride(0) if rows > 1 else kb, w_stride,
-                weight_scale.stride(0) if n > FP8_GROUP else kb, out.stride(0) if rows > 1 else n,
-                _DTYPES[out_dtype], _status_ptr(status), _stream(dev)),
-        )
+    _call(dev, "pkv_linear_fp8", x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(),
+          _lib.ptr(bias), out.data_ptr(), rows, n, k, x_stride, x_scale.stride(0) if rows > 1 else kb, w_stride,
+          weight_scale.stride(0) if n > FP8_GROUP else kb, out.stride(0) if rows > 1 else n, _DTYPES[out_dtype],
+          _status_ptr(status))
     return out
 
 
@@ -885,6 +883,17 @@ def _check_logits(logits: torch.Tensor, tokens: torch.Tensor, temperature: float
         raise ValueError("temperature must be > 0.")
 
 
+def _tokens64(tokens: torch.Tensor) -> torch.Tensor:
+    return (tokens if tokens.dtype == torch.int64 else tokens.to(torch.int64)).contiguous()
+
+
+def _f32(t: torch.Tensor) -> torch.Tensor:
+    """t as an fp32 constant."""
+    if t.requires_grad:
+        t = t.detach()
+    return t if t.dtype == torch.float32 else t.to(torch.float32)
+
+
 def _first_order(what: str) -> None:
     # (grad mode is on in a backward pass under create_graph; once_differentiable says the same, 20 us later)
     if torch.is_grad_enabled():
@@ -894,17 +903,12 @@ def _first_order(what: str) -> None:
 def _logprobs_forward(logits, tokens, temperature, entropy, want_stats, status):
     logits, rows, inner, outer_stride, row_stride = _logit_rows(logits)
     dev = logits.device
-    logp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    logp = torch.empty_like(tokens, dtype=torch.float32)
     ent = torch.empty_like(logp) if entropy else None
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None
-    with _device_ctx(dev):
-        _lib.check(
-            "pkv_token_logprobs",
-            _lib.load().pkv_token_logprobs(
-                logits.data_ptr(), _DTYPES[logits.dtype], tokens.data_ptr(), rows, logits.shape[-1], inner,
-                outer_stride, row_stride, temperature, logp.data_ptr(), _lib.ptr(ent), _lib.ptr(stats),
-                _status_ptr(status), _stream(dev)),
-        )
+    stats = _empty2(rows, 2, torch.float32, dev) if want_stats else None
+    _call(dev, "pkv_token_logprobs", logits.data_ptr(), _DTYPES[logits.dtype], tokens.data_ptr(), rows,
+          logits.shape[-1], inner, outer_stride, row_stride, temperature, logp.data_ptr(), _lib.ptr(ent),
+          _lib.ptr(stats), _status_ptr(status))
     return logp, ent, stats
 
 
@@ -927,14 +931,9 @@ class _TokenLogprobs(torch.autograd.Function):
         dev = src.device
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         d_logp, d_ent = (None if d is None else d.contiguous() for d in (d_logp, d_ent))
-        with _device_ctx(dev):
-            _lib.check(
-                "pkv_token_logprobs_grad",
-                _lib.load().pkv_token_logprobs_grad(
-                    src.data_ptr(), _DTYPES[src.dtype], tokens.data_ptr(), rows, src.shape[-1], inner, outer_stride,
-                    row_stride, ctx.temperature, stats.data_ptr(), _lib.ptr(ent), _lib.ptr(d_logp), _lib.ptr(d_ent),
-                    grad.data_ptr(), _stream(dev)),
-            )
+        _call(dev, "pkv_token_logprobs_grad", src.data_ptr(), _DTYPES[src.dtype], tokens.data_ptr(), rows,
+              src.shape[-1], inner, outer_stride, row_stride, ctx.temperature, stats.data_ptr(), _lib.ptr(ent),
+              _lib.ptr(d_logp), _lib.ptr(d_ent), grad.data_ptr())
         return grad, None, None, None, None
 
 
@@ -958,7 +957,7 @@ def token_logprobs(
     _check_logits(logits, tokens, temperature, (2, 3))
     _dtype_code(logits, "logits")
     _require_cuda(logits, tokens, status)
-    tokens = tokens.to(torch.int64).contiguous()
+    tokens = _tokens64(tokens)
     if logits.requires_grad and torch.is_grad_enabled():
         return _TokenLogprobs.apply(logits, tokens, float(temperature), bool(entropy), status)
     logp, ent, _ = _logprobs_forward(logits, tokens, float(temperature), entropy, False, status)
@@ -982,28 +981,23 @@ def _policy_forward(logits, tokens, old, ref, adv, mask, kl_coef, clip_low, clip
     src, rows, _, batch_stride, row_stride = _logit_rows(logits)
     batch, length, vocab = logits.shape
     dev = logits.device
-    lib = _lib.load()
-    out = torch.empty(3, dtype=torch.float32, device=dev)
+    out = torch.empty_strided((3,), (1,), dtype=torch.float32, device=dev)
     logp = _empty2(batch, length, torch.float32, dev)
-    ws = torch.empty(lib.pkv_policy_loss_workspace_size(batch, length), dtype=torch.uint8, device=dev)
+    ws_bytes = _lib.load().pkv_policy_loss_workspace_size(batch, length)
+    ws = torch.empty_strided((ws_bytes,), (1,), dtype=torch.uint8, device=dev)
     grad = None
     if want_grad:
         grad = torch.empty_strided((batch, length, vocab), (length * vocab, vocab, 1), dtype=logits.dtype, device=dev)
-    with _device_ctx(dev):
-        _lib.check(
-            "pkv_policy_loss",
-            lib.pkv_policy_loss(
-                src.data_ptr(), _DTYPES[src.dtype], tokens.data_ptr(), old.data_ptr(), _lib.ptr(ref), adv.data_ptr(),
-                adv.stride(0), adv.stride(1) if adv.ndim == 2 else 0, _lib.ptr(mask), batch, length, vocab,
-                batch_stride, row_stride, temperature, clip_low, clip_high, kl_coef, reduction, out.data_ptr(),
-                logp.data_ptr(), _lib.ptr(grad), ws.data_ptr(), ws.numel(), _status_ptr(status), _stream(dev)),
-        )
+    _call(dev, "pkv_policy_loss", src.data_ptr(), _DTYPES[src.dtype], tokens.data_ptr(), old.data_ptr(),
+          _lib.ptr(ref), adv.data_ptr(), adv.stride(0), adv.stride(1) if adv.ndim == 2 else 0, _lib.ptr(mask), batch,
+          length, vocab, batch_stride, row_stride, temperature, clip_low, clip_high, kl_coef, reduction,
+          out.data_ptr(), logp.data_ptr(), _lib.ptr(grad), ws.data_ptr(), ws_bytes, _status_ptr(status))
     return out[0], logp, out[1], out[2], grad
 
 
 class _PolicyLossFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, *args):
+    def forward(ctx, logits, args):  # (one argument for all constants: apply looks at each)
         loss, logp, kl, clipped, ctx.d_logits = _policy_forward(logits, *args, True)
         ctx.mark_non_differentiable(logp, kl, clipped)
         ctx.set_materialize_grads(False)  # (no zeros for the outputs without a gradient)
@@ -1013,17 +1007,13 @@ class _PolicyLossFn(torch.autograd.Function):
     def backward(ctx, d_loss, *unused):
         _first_order("policy_loss")
         if d_loss is None:
-            return (None,) * 12
+            return None, None
         grad, ctx.d_logits = ctx.d_logits, None
         if grad is None:
             raise RuntimeError("policy_loss: its gradient was computed with the loss and has been handed out; call "
                                "policy_loss again for another backward pass.")
-        dev = grad.device
-        with _device_ctx(dev):
-            _lib.check("pkv_scale_grad", _lib.load().pkv_scale_grad(grad.data_ptr(), grad.numel(),
-                                                                    _DTYPES[grad.dtype], d_loss.data_ptr(),
-                                                                    _stream(dev)))
-        return (grad,) + (None,) * 11
+        _call(grad.device, "pkv_scale_grad", grad.data_ptr(), grad.numel(), _DTYPES[grad.dtype], d_loss.data_ptr())
+        return grad, None
 
 
 def policy_loss(
@@ -1078,14 +1068,14 @@ def policy_loss(
     if mask is not None:
         mask = (mask if mask.dtype in (torch.bool, torch.uint8) else mask != 0).contiguous()
     args = (
-        tokens.to(torch.int64).contiguous(),
-        old_logprobs.detach().to(torch.float32).contiguous(),
-        None if ref_logprobs is None else ref_logprobs.detach().to(torch.float32).contiguous(),
-        advantages.detach().to(torch.float32),
+        _tokens64(tokens),
+        _f32(old_logprobs).contiguous(),
+        None if ref_logprobs is None else _f32(ref_logprobs).contiguous(),
+        _f32(advantages),
         mask, float(kl_coef), float(clip_low), float(clip_high), float(temperature), _REDUCTIONS[reduction], status,
     )
     if logits.requires_grad and torch.is_grad_enabled():
-        return PolicyLoss(*_PolicyLossFn.apply(logits, *args))
+        return PolicyLoss(*_PolicyLossFn.apply(logits, args))
     return PolicyLoss(*_policy_forward(logits, *args, False)[:4])
 
 
