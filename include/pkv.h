@@ -2,7 +2,9 @@
  * pkv.h — C ABI of the B200 paged-KV library (libpkv.so).
  *
  * The library implements the rollout hot path of the GRPO trainer: the paged
- * KV-cache page append and the paged-KV (GQA) single-query decode attention.
+ * KV-cache page append and the paged-KV (GQA) single-query decode attention,
+ * the steps around them, and what a policy update does with a rollout: scoring
+ * in 8 bits, token log-probabilities and the clipped policy loss (at the end).
  * Every entry point takes plain device pointers, element strides and sizes,
  * enqueues its kernels on the given CUDA stream (a cudaStream_t passed as
  * void*; NULL = legacy default stream) and returns without synchronising.
