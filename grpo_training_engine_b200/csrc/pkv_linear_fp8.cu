@@ -127,6 +127,13 @@ __device__ __forceinline__ void tma_load_group(void *dst, const CUtensorMap *map
         : "memory");
 }
 
+// One lane of the (converged) warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
 // Bounded wait of a thread that others wait for in turn: it looks again at once.
 __device__ __forceinline__ bool mbar_wait_spin(uint64_t *bar, uint32_t parity, uint32_t max_polls) {
   for (uint32_t i = 0; i < max_polls; ++i)
@@ -305,35 +312,34 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
 
   if (warp < kFirstEpi) {
     if constexpr (kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    // (Warps 0 and 1 run their loops whole, one lane issues: the descriptors then are uniform values.)
     if (warp == 0) {
-      if (lane == 0) {
-        int i = 0, issued = 0;
-        bool ok = true;
-        for (int t = first; t < tiles && ok; t += step) {
-          const int m0 = tile_m(t), n0 = tile_n(t) + rank * (BN / G);
-          for (int k = 0; k < nkb; ++k, ++i) {
-            const int s = i % S, use = i / S;
-            if (use > 0 && !mbar_wait_spin(&empty[s], (use - 1) & 1, a.max_polls)) {
-              flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
-              ok = false;
-              break;
-            }
+      int i = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        const int m0 = tile_m(t), n0 = tile_n(t) + rank * (BN / G);
+        for (int k = 0; k < nkb; ++k, ++i) {
+          const int s = i % S, use = i / S;
+          ok = __all_sync(0xffffffffu, use == 0 || mbar_wait_spin(&empty[s], (use - 1) & 1, a.max_polls));
+          if (!ok) break;
+          if (elect_one()) {
             uint32_t bar = smem_u32(&full[s]);
             if (G == 2) bar = map_cluster(bar, 0);
             if (rank == 0) mbar_expect_tx(&full[s], G * (a.x_rows * kBK + L::kB));
             tma_load_group<G>(sa + s * L::kA, &tx, (kb0 + k) * kBK, m0, bar);
             tma_load_group<G>(sb + s * L::kB, &tw, (kb0 + k) * kBK, n0, bar);
-            ++issued;
           }
+          __syncwarp();
         }
-        // the last load of each stage has landed before the shared memory goes away (in the pair's second
-        // CTA: the MMAs that read it are waited for)
-        if (rank == 0)
-          for (int j = issued > S ? issued - S : 0; j < issued; ++j)
-            if (!mbar_wait_spin(&full[j % S], (j / S) & 1, a.max_polls)) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
       }
+      if (!ok) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
+      // the last load of each stage has landed before the shared memory goes away (in the pair's second
+      // CTA: the MMAs that read it are waited for)
+      if (rank == 0)
+        for (int j = i > S ? i - S : 0; j < i; ++j)
+          if (!mbar_wait_spin(&full[j % S], (j / S) & 1, a.max_polls)) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
     } else if (warp == 1) {
-      if (lane == 0 && rank == 0) {
+      if (rank == 0) {
         constexpr uint32_t idesc = f8_idesc(kBM * G, BN);
         int i = 0;
         bool ok = true;
@@ -342,20 +348,23 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
             const int s = i % S, buf = i % NB, use = i / NB;
             ok = mbar_wait_spin(&full[s], (i / S) & 1, a.max_polls) &&
                  (use == 0 || mbar_wait_spin(&acc_empty[buf], (use - 1) & 1, a.max_polls));
-            if (!ok) {
-              flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
-              break;
-            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
             tc_fence_after();
             const uint64_t ad = sw128_desc(sa + s * L::kA), bd = sw128_desc(sb + s * L::kB);
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kBK / 32; ++kk)  // 32 bytes of k per MMA along the swizzled rows
-              tc_mma_f8<G>(tmem + buf * BN, ad + 2 * kk, bd + 2 * kk, idesc, kk > 0 ? 1u : 0u);
-            tc_commit_group<G>(&acc_full[buf]);
-            tc_commit_group<G>(&empty[s]);
+              for (int kk = 0; kk < kBK / 32; ++kk)  // 32 bytes of k per MMA along the swizzled rows
+                tc_mma_f8<G>(tmem + buf * BN, ad + 2 * kk, bd + 2 * kk, idesc, kk > 0 ? 1u : 0u);
+              tc_commit_group<G>(&acc_full[buf]);
+              tc_commit_group<G>(&empty[s]);
+            }
+            __syncwarp();
           }
         }
-        tc_commit_group<G>(done);
+        if (!ok) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
+        if (elect_one()) tc_commit_group<G>(done);
+        __syncwarp();
       }
     } else if (warp == 2) {
       // four blocks at a time, the next four's loads in flight while these are handed out
