@@ -146,7 +146,7 @@ __host__ __device__ constexpr uint32_t f8_idesc(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// 32 or 16 columns of this thread's TMEM lane; the values are there after tmem_wait.
+// 32 columns of this thread's TMEM lane; the values are there after tmem_wait.
 __device__ __forceinline__ void tmem_ld_async(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -157,21 +157,7 @@ __device__ __forceinline__ void tmem_ld_async(uint32_t taddr, uint32_t (&v)[32])
         "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld_async(uint32_t taddr, uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr));
-}
 // Waits for this thread's loads; passing the registers through keeps their uses behind it.
-__device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
-                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
-               :
-               : "memory");
-}
 __device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
@@ -197,11 +183,10 @@ __device__ __forceinline__ void fma_cols(float2 (&acc)[N / 2], const uint32_t (&
 __device__ __forceinline__ uint32_t bits16(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 __device__ __forceinline__ uint32_t bits16(__half v) { return __half_as_ushort(v); }
 
-// P CTAs share an SM.
-template <int BN, int S, int G, int P>
+template <int BN, int S, int G>
 struct Smem {
   static constexpr int kA = kBM * kBK, kB = BN / G * kBK;  // one stage of x and of W, bytes
-  static constexpr int kCols = 512 / P;                    // TMEM columns
+  static constexpr int kCols = 512;                        // TMEM columns: all
   static constexpr int kBufs = kCols / BN;                 // TMEM buffers of BN fp32 columns
   static constexpr int kCW = BN / 2;                       // columns of an epilogue warp
   static constexpr int kBlocks = (BN + 127) / 128;         // blocks of W's scales across a tile
@@ -247,12 +232,12 @@ __device__ __forceinline__ void store_cols(const Fp8Args &a, int row, int col, c
     if (col + j < a.n) out[j] = o[j];
 }
 
-template <typename T, int BN, int S, int G, int P>
-__global__ void __launch_bounds__(kThreads, P)
+template <typename T, int BN, int S, int G>
+__global__ void __launch_bounds__(kThreads, 1)
 linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
                   const __grid_constant__ CUtensorMap to, Fp8Args a) {
-  using L = Smem<BN, S, G, P>;
-  constexpr int NB = L::kBufs, CW = L::kCW, ST = CW >= 64 ? 32 : 16;
+  using L = Smem<BN, S, G>;
+  constexpr int NB = L::kBufs, CW = L::kCW, ST = 32;
   constexpr bool kSplitRegs = CW == 128;  // 128 sums per epilogue thread
   extern __shared__ uint8_t raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -590,10 +575,10 @@ int encode_rows(CUtensorMap *map, CUtensorMapDataType type, int size, const void
   return PKV_OK;
 }
 
-template <typename T, int BN, int S, int G, int P>
+template <typename T, int BN, int S, int G>
 int fp8_launch(const void *x, const void *w, int64_t k, int64_t x_stride, int64_t w_stride, Fp8Args a,
                cudaStream_t st) {
-  using L = Smem<BN, S, G, P>;
+  using L = Smem<BN, S, G>;
   static_assert(L::kBytes <= 227 * 1024, "shared memory");
   static_assert(G == 2 || kBM * (BN + 4) * sizeof(float) <= L::kSc, "the split tile fits the ring");
   a.x_rows = std::min(kBM, (a.rows + 7) / 8 * 8);
@@ -605,13 +590,13 @@ int fp8_launch(const void *x, const void *w, int64_t k, int64_t x_stride, int64_
   if (rc == PKV_OK && a.tma_out)
     rc = encode_rows(&to, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, a.out, a.n, a.rows, a.out_stride, 32);
   if (rc != PKV_OK) return rc;
-  auto kern = linear_fp8_kernel<T, BN, S, G, P>;
+  auto kern = linear_fp8_kernel<T, BN, S, G>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes) != cudaSuccess)
     return check_launch("cudaFuncSetAttribute(linear_fp8)");
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
   const int cluster = G == 2 ? 2 : a.splits;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min<int64_t>(tiles * cluster, lin_sms() * P / cluster * cluster));
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(tiles * cluster, lin_sms() / cluster * cluster));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = L::kBytes;
   cfg.stream = st;
@@ -639,14 +624,18 @@ int fp8_dispatch(const void *x, const void *w, int64_t k, int64_t x_stride, int6
   // Many rows: pairs, whose 256 x 256 tiles read least from L2 for what they multiply (4096 x 18944 x 3584: 336 us
   // against 426 with 128 x 128 tiles, which stop at 10 TB/s out of L2).
   if (a.rows > kBM && tiles(256, 256) >= sms / 2)
-    return fp8_launch<T, 256, 4, 2, 1>(x, w, k, x_stride, w_stride, a, st);
+    return fp8_launch<T, 256, 4, 2>(x, w, k, x_stride, w_stride, a, st);
   // Wide matrices: an MMA of 256 columns takes little longer than one of 64 (151,936 columns by 37 rows: 54 us
   // against 67).
-  if (tiles(128, 256) >= 2 * sms) return fp8_launch<T, 256, 4, 1, 1>(x, w, k, x_stride, w_stride, a, st);
-  // The rest: narrow tiles, two CTAs on an SM, k split until they fill the machine.
-  const int64_t t = tiles(128, 64);
-  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)a.kblocks, (int64_t)kMaxSplits, 2 * sms / t}));
-  return fp8_launch<T, 64, 4, 1, 2>(x, w, k, x_stride, w_stride, a, st);
+  if (tiles(128, 256) >= 2 * sms) return fp8_launch<T, 256, 4, 1>(x, w, k, x_stride, w_stride, a, st);
+  // The rest: 128-column tiles, k split until they fill the machine. (Twice as many of 64 columns, two CTAs on an SM,
+  // took 12.0 us for 128 x 1536 x 8960 where this takes 11.7, 10.2 against 8.2 for 24 x 8960 x 1536.) Clusters of
+  // more than 4 only where all of them fit at once: 16 of 8 did not, and took a second round (2048 x 1536: 11.8 us).
+  const int64_t t = tiles(128, 128);
+  int64_t splits = std::min<int64_t>({(int64_t)a.kblocks, (int64_t)kMaxSplits, sms / t});
+  if (splits > 4 && t * splits > 96) splits = 4;
+  a.splits = (int)std::max<int64_t>(1, splits);
+  return fp8_launch<T, 128, 6, 1>(x, w, k, x_stride, w_stride, a, st);
 }
 
 }  // namespace
