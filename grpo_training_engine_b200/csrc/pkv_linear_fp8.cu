@@ -192,8 +192,7 @@ struct Smem {
   static constexpr int kBlocks = (BN + 127) / 128;         // blocks of W's scales across a tile
   static constexpr size_t kW = (size_t)S * kA;
   static constexpr size_t kOut = kW + (size_t)S * kB;      // 32 rows x kCW 16-bit results of each epilogue warp
-  static constexpr bool kStage = G == 2;                   // (few rows: direct stores)
-  static constexpr size_t kSc = kOut + (kStage ? kEpiWarps * 32 * kCW * 2 : 0);  // [kBufs][kBlocks][kBM] fp32
+  static constexpr size_t kSc = kOut + kEpiWarps * 32 * kCW * 2;  // [kBufs][kBlocks][kBM] fp32
   static constexpr size_t kFull = kSc + 4 * kBufs * kBlocks * kBM;
   static constexpr size_t kEmpty = kFull + 8 * S;
   static constexpr size_t kAccFull = kEmpty + 8 * S;
@@ -465,7 +464,7 @@ linear_fp8_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant_
         scale = next;
       }
       if (!ok) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
-      if (L::kStage && a.splits == 1 && a.tma_out) {
+      if (a.splits == 1 && a.tma_out) {
         // 32 rows by 64 columns at a time, swizzled as TMA reads them, which clips what lies outside
         const int row0 = row - lane;
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last tile's have been read
@@ -586,7 +585,7 @@ int fp8_launch(const void *x, const void *w, int64_t k, int64_t x_stride, int64_
   int rc = encode_rows(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, k, a.rows, x_stride, a.x_rows);
   if (rc == PKV_OK) rc = encode_rows(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, k, a.n, w_stride, BN / G);
   to = tx;
-  a.tma_out = L::kStage && aligned_to(a.out, 16) && a.out_stride % 8 == 0;
+  a.tma_out = aligned_to(a.out, 16) && a.out_stride % 8 == 0;
   if (rc == PKV_OK && a.tma_out)
     rc = encode_rows(&to, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, a.out, a.n, a.rows, a.out_stride, 32);
   if (rc != PKV_OK) return rc;
@@ -623,19 +622,21 @@ int fp8_dispatch(const void *x, const void *w, int64_t k, int64_t x_stride, int6
   a.splits = 1;
   // Many rows: pairs, whose 256 x 256 tiles read least from L2 for what they multiply (4096 x 18944 x 3584: 336 us
   // against 426 with 128 x 128 tiles, which stop at 10 TB/s out of L2).
-  if (a.rows > kBM && tiles(256, 256) >= sms / 2)
+  if (a.rows > kBM && tiles(256, 256) >= sms / 4)
     return fp8_launch<T, 256, 4, 2>(x, w, k, x_stride, w_stride, a, st);
   // Wide matrices: an MMA of 256 columns takes little longer than one of 64 (151,936 columns by 37 rows: 54 us
   // against 67).
-  if (tiles(128, 256) >= 2 * sms) return fp8_launch<T, 256, 4, 1>(x, w, k, x_stride, w_stride, a, st);
+  if (tiles(128, 256) >= 2 * sms) return fp8_launch<T, 256, 3, 1>(x, w, k, x_stride, w_stride, a, st);
   // The rest: 128-column tiles, k split until they fill the machine. (Twice as many of 64 columns, two CTAs on an SM,
   // took 12.0 us for 128 x 1536 x 8960 where this takes 11.7, 10.2 against 8.2 for 24 x 8960 x 1536.) Clusters of
-  // more than 4 only where all of them fit at once: 16 of 8 did not, and took a second round (2048 x 1536: 11.8 us).
+  // more than 2 only where all of them fit at once: 16 of 8 did not and took a second round (2048 x 1536: 11.8 us, 6.7
+  // in clusters of 4), nor 48 of 3 (512 x 1536 x 8960: 33 us).
   const int64_t t = tiles(128, 128);
   int64_t splits = std::min<int64_t>({(int64_t)a.kblocks, (int64_t)kMaxSplits, sms / t});
   if (splits > 4 && t * splits > 96) splits = 4;
+  while (splits > 2 && t * splits > 120) --splits;
   a.splits = (int)std::max<int64_t>(1, splits);
-  return fp8_launch<T, 128, 6, 1>(x, w, k, x_stride, w_stride, a, st);
+  return fp8_launch<T, 128, 5, 1>(x, w, k, x_stride, w_stride, a, st);
 }
 
 }  // namespace
