@@ -29,7 +29,7 @@
 // of a cluster, which add their fp32 tiles in split order through distributed
 // shared memory, so results do not depend on timing.
 //
-// Bounds. 4096 x 18944 x 3584: 339 us, 1640 TFLOP/s (a bf16 library product of
+// Bounds. 4096 x 18944 x 3584: 322 us, 1730 TFLOP/s (a bf16 library product of
 // 8192^3 reaches 1634 here). The tensor pipe is busy 36% of the time: a block's
 // sums have to be out of TMEM before its buffer is filled again, and all 512
 // columns hold two blocks of a pair's tile. Leaving the epilogue's reads out
@@ -37,7 +37,8 @@
 // core (wrong scales) 0.52. 128 x 128 tiles by single CTAs stop at 426 us, 10
 // TB/s out of L2; two MMAs of 128 columns per block take 0.88 us a block; 16
 // epilogue warps of 64 columns 433 us (96 registers each). 37 x 151,936 x 1536:
-// 55 us, 4.4 TB/s of weights, bound by the same hand-over of 12-block tiles.
+// 54 us, 4.5 TB/s of weights: 594 tiles of 12 blocks, two more than four rounds,
+// each with the same hand-over. 128 x 1536 x 8960: 12 us, mostly set-up.
 //
 // Every wait is bounded; one that runs out sets PKV_DEV_WAIT_TIMEOUT, and the
 // CTA waits (bounded) for its own copies and MMAs, frees its TMEM and returns.
@@ -620,8 +621,9 @@ int fp8_dispatch(const void *x, const void *w, int64_t k, int64_t x_stride, int6
     return (int64_t)a.tiles_m * a.tiles_n;
   };
   a.splits = 1;
-  // Many rows: pairs, whose 256 x 256 tiles read least from L2 for what they multiply (4096 x 18944 x 3584: 336 us
-  // against 426 with 128 x 128 tiles, which stop at 10 TB/s out of L2).
+  // Many rows: pairs, whose 256 x 256 tiles read least from L2 for what they multiply (4096 x 18944 x 3584: 322 us
+  // against 426 with 128 x 128 tiles, which stop at 10 TB/s out of L2), from half a round of them on (512 x 8960 x
+  // 1536: 15.2 us against 18.1).
   if (a.rows > kBM && tiles(256, 256) >= sms / 4)
     return fp8_launch<T, 256, 4, 2>(x, w, k, x_stride, w_stride, a, st);
   // Wide matrices: an MMA of 256 columns takes little longer than one of 64 (151,936 columns by 37 rows: 54 us
