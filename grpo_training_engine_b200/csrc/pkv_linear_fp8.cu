@@ -30,15 +30,16 @@
 // shared memory, so results do not depend on timing.
 //
 // Bounds. 4096 x 18944 x 3584: 322 us, 1730 TFLOP/s (a bf16 library product of
-// 8192^3 reaches 1634 here). The tensor pipe is busy 36% of the time: a block's
+// 8192^3 reaches 1634 here). The tensor pipe is busy 38% of the time: a block's
 // sums have to be out of TMEM before its buffer is filled again, and all 512
-// columns hold two blocks of a pair's tile. Leaving the epilogue's reads out
-// gives 0.64 us a block instead of 0.67, adding 28 blocks up inside the tensor
-// core (wrong scales) 0.52. 128 x 128 tiles by single CTAs stop at 426 us, 10
-// TB/s out of L2; two MMAs of 128 columns per block take 0.88 us a block; 16
-// epilogue warps of 64 columns 433 us (96 registers each). 37 x 151,936 x 1536:
-// 54 us, 4.5 TB/s of weights: 594 tiles of 12 blocks, two more than four rounds,
-// each with the same hand-over. 128 x 1536 x 8960: 12 us, mostly set-up.
+// columns hold two blocks of a pair's tile. Measured in an earlier form of 339
+// us: leaving the epilogue's reads out gave 0.64 us a block instead of 0.67,
+// adding 28 blocks up inside the tensor core (wrong scales) 0.52; 128 x 128
+// tiles by single CTAs stopped at 426 us, 10 TB/s out of L2; two MMAs of 128
+// columns per block took 0.88 us a block; 16 epilogue warps of 64 columns 433 us
+// (96 registers each). 37 x 151,936 x 1536: 54 us, 4.3 TB/s of weights: 594
+// tiles of 12 blocks, two more than four rounds, each with the same hand-over.
+// 128 x 1536 x 8960: 11.8 us; with k = 1024, one block per split, 8.3.
 //
 // Every wait is bounded; one that runs out sets PKV_DEV_WAIT_TIMEOUT, and the
 // CTA waits (bounded) for its own copies and MMAs, frees its TMEM and returns.
@@ -623,7 +624,7 @@ int fp8_dispatch(const void *x, const void *w, int64_t k, int64_t x_stride, int6
   a.splits = 1;
   // Many rows: pairs, whose 256 x 256 tiles read least from L2 for what they multiply (4096 x 18944 x 3584: 322 us
   // against 426 with 128 x 128 tiles, which stop at 10 TB/s out of L2), from half a round of them on (512 x 8960 x
-  // 1536: 15.2 us against 18.1).
+  // 1536: 15.6 us against 18.1).
   if (a.rows > kBM && tiles(256, 256) >= sms / 4)
     return fp8_launch<T, 256, 4, 2>(x, w, k, x_stride, w_stride, a, st);
   // Wide matrices: an MMA of 256 columns takes little longer than one of 64 (151,936 columns by 37 rows: 54 us
