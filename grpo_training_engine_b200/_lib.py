@@ -124,6 +124,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pkv_policy_loss": (C.c_int, [_vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i64, _i64,
                                   C.c_float, C.c_float, C.c_float, C.c_float, _i32, _vp, _vp, _vp, _vp, _sz, _vp,
                                   _vp]),
+    "pkv_policy_loss_grad": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i64, _i64, C.c_float, _vp, _sz, _vp, _vp, _vp]),
     "pkv_scale_grad": (C.c_int, [_vp, _i64, _i32, _vp, _vp]),
 }
 

@@ -479,6 +479,7 @@ struct PolicyArgs {
   int32_t *order;          // workspace [batch * length]: tokens with a weight first
   int32_t *before;         // workspace [batch + 1]: such tokens before each sequence
   int32_t *counts;         // workspace: [0] tokens with a weight, [1] blocks done
+  float4 *slopes;          // workspace [batch * length], or nullptr: what policy_grad_scaled_kernel takes of a row
   int32_t *status;
   int64_t adv_b, adv_t;
   int32_t batch, length, vocab, reduction;
@@ -605,7 +606,9 @@ __device__ __forceinline__ RowResult token_result(const PolicyArgs &a, const Tok
                   : a.reduction == PKV_REDUCE_SEQUENCE ? 1.f / ((float)t.len * (float)a.batch)
                                                        : 1.f / (float)t.len;
   slope *= w * a.inv_t;
-  return RowResult{st.m, -slope / st.s, slope, t.tok};
+  const RowResult res{st.m, -slope / st.s, slope, t.tok};
+  if (a.slopes != nullptr) a.slopes[r] = make_float4(res.m, res.k, res.slope, __int_as_float(t.in ? (int)t.tok : -1));
+  return res;
 }
 
 // Called by the NT threads of a block with its sums in thread 0: the block that
@@ -933,6 +936,34 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
   finish<NT + 32>(a, sums, blockIdx.x, gridDim.x);
 }
 
+// The gradient again, for an upstream u other than 1, from what the loss kept of
+// each row: u enters the fp32 slope, so an element is rounded once, where the
+// stored gradient times u would have been rounded twice, and an fp16 element below
+// the type's smallest step would have been lost before a loss scale could lift it.
+// Nothing to do where u is 1, or in a row whose gradient is zero (no weight, or
+// clipped): policy_loss wrote that. NT threads per row, or per share of one (ctas of
+// them, no larger than 64 KB); a persistent grid, since a launch for u = 1 should
+// cost no more than a launch.
+template <typename T, int NT>
+__global__ void __launch_bounds__(kThreads, 4)
+policy_grad_scaled_kernel(const T *logits, Rows rows, T *grad, const float4 *slopes, const int32_t *order,
+                          const int32_t *counts, const float *upstream, int32_t vocab, int32_t ctas, float c) {
+  const float u = *upstream;
+  if (u == 1.f) return;
+  const int64_t items = (int64_t)counts[0] * ctas, step = gridDim.x * (int64_t)(kThreads / NT);
+  const int tid = threadIdx.x % NT;
+  for (int64_t at = blockIdx.x * (int64_t)(kThreads / NT) + threadIdx.x / NT; at < items; at += step) {
+    const int64_t r = order[at / ctas];
+    const float4 st = slopes[r];
+    if (st.y == 0.f && st.z == 0.f) continue;
+    const Slice<T> sl(logits + rows.offset(r), vocab, (int)(at % ctas), ctas);
+    const Slope g{st.x, c, st.y * u, 0.f, st.z * u, __float_as_int(st.w)};
+    T *out = grad + r * (int64_t)vocab;
+    grad_range<T, false, NT>(sl, g, out, sl.vecs() + sl.lo, sl.lo, sl.hi, tid);
+    grad_edge<T, false>(sl, g, out, tid);
+  }
+}
+
 // grad *= *upstream, nothing where it is 1
 template <typename T>
 __global__ void __launch_bounds__(kThreads) scale_grad_kernel(T *grad, int64_t n, const float *upstream) {
@@ -1009,6 +1040,22 @@ int launch_grad(const T *logits, Rows rows, T *grad, const PolicyArgs &a, void *
   // in one, of 200 KB 167 us for 2048 in two and 175 in one, of 304 KB 568 us for 4096 in two and 481 in one.
   if (bytes <= 200 * 1024) return launch_held<T, 384, 4, 2>(logits, rows, grad, a, stream);
   return launch_held<T, 896, 3, 1>(logits, rows, grad, a, stream);
+}
+
+// The parts of a policy loss's workspace: the blocks' sums, two counters, what a
+// scaled gradient takes of a row, an index per token, a count per sequence.
+struct PolicyWorkspace {
+  size_t counts, slopes, order, before, bytes;
+};
+PolicyWorkspace policy_workspace(int32_t batch, int32_t length) {
+  const size_t rows = (size_t)batch * length;
+  PolicyWorkspace w;
+  w.counts = kMaxBlocks * 24;
+  w.slopes = w.counts + 16;
+  w.order = w.slopes + rows * sizeof(float4);
+  w.before = w.order + rows * 4;
+  w.bytes = w.before + ((size_t)batch + 1) * 4;
+  return w;
 }
 
 bool bad_logits(const char *fn, const void *logits, int32_t dtype, int64_t rows, int32_t vocab, int32_t inner,
@@ -1090,8 +1137,7 @@ extern "C" int pkv_token_logprobs_grad(const void *logits, int32_t dtype, const 
 
 extern "C" size_t pkv_policy_loss_workspace_size(int32_t batch, int32_t length) {
   if (batch < 0 || length < 0 || (int64_t)batch * length > INT32_MAX) return 0;
-  // the blocks' sums, two counters, an index per token, a count per sequence
-  return kMaxBlocks * 24 + 16 + ((size_t)batch * length + batch + 1) * 4;
+  return policy_workspace(batch, length).bytes;
 }
 
 extern "C" int pkv_policy_loss(const void *logits, int32_t dtype, const int64_t *tokens, const float *old_logprobs,
@@ -1128,10 +1174,12 @@ extern "C" int pkv_policy_loss(const void *logits, int32_t dtype, const int64_t 
   a.out = out;
   a.logp = logprobs;
   uint8_t *ws = static_cast<uint8_t *>(workspace);
+  const PolicyWorkspace w = policy_workspace(batch, length);
   a.partial = reinterpret_cast<double *>(ws);
-  a.counts = reinterpret_cast<int32_t *>(ws + kMaxBlocks * 24);
-  a.order = a.counts + 4;
-  a.before = a.order + rows;
+  a.counts = reinterpret_cast<int32_t *>(ws + w.counts);
+  a.slopes = d_logits ? reinterpret_cast<float4 *>(ws + w.slopes) : nullptr;
+  a.order = reinterpret_cast<int32_t *>(ws + w.order);
+  a.before = reinterpret_cast<int32_t *>(ws + w.before);
   a.status = status;
   a.adv_b = adv_stride_b;
   a.adv_t = adv_stride_t;
@@ -1159,6 +1207,42 @@ extern "C" int pkv_policy_loss(const void *logits, int32_t dtype, const int64_t 
                                            a))
   }
   return PKV_ERR_UNSUPPORTED;
+}
+
+extern "C" int pkv_policy_loss_grad(const void *logits, int32_t dtype, int32_t batch, int32_t length, int32_t vocab,
+                                    int64_t batch_stride, int64_t row_stride, float temperature,
+                                    const void *workspace, size_t workspace_bytes, const float *upstream,
+                                    void *d_logits, void *stream) {
+  if (dtype_size(dtype) == 0) return PKV_ERR_UNSUPPORTED;
+  const int64_t rows = (int64_t)batch * length;
+  if (batch < 0 || length < 0 ||
+      bad_logits("pkv_policy_loss_grad", logits, dtype, rows, vocab, std::max(1, length), temperature))
+    return PKV_ERR_INVALID_ARG;
+  if (rows == 0) return PKV_OK;
+  if (!upstream || !d_logits || !aligned_to(upstream, 4) || !aligned_to(d_logits, dtype_size(dtype))) {
+    set_error_detail("pkv_policy_loss_grad: NULL or misaligned pointer");
+    return PKV_ERR_INVALID_ARG;
+  }
+  const PolicyWorkspace w = policy_workspace(batch, length);
+  if (!workspace || workspace_bytes < w.bytes || !aligned_to(workspace, 16)) return PKV_ERR_WORKSPACE;
+  const uint8_t *ws = static_cast<const uint8_t *>(workspace);
+  const auto *counts = reinterpret_cast<const int32_t *>(ws + w.counts);
+  const auto *slopes = reinterpret_cast<const float4 *>(ws + w.slopes);
+  const auto *order = reinterpret_cast<const int32_t *>(ws + w.order);
+  const Rows rw{batch_stride, row_stride, length};
+  const int64_t bytes = (int64_t)vocab * dtype_size(dtype);
+  const bool warps = warp_rows(rows, bytes);
+  const int ctas = warps ? 1 : row_ctas(rows, bytes, 64 * 1024);
+  const unsigned blocks =
+      (unsigned)std::min<int64_t>(warps ? (rows - 1) / kWarps + 1 : rows * ctas, 148 * 4);
+  const float c = (float)(kLog2e / temperature);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  PKV_BY_DTYPE(dtype, {
+    auto k = warps ? policy_grad_scaled_kernel<T, 32> : policy_grad_scaled_kernel<T, kThreads>;
+    k<<<blocks, kThreads, 0, st>>>((const T *)logits, rw, (T *)d_logits, slopes, order, counts, upstream, vocab, ctas,
+                                   c);
+  })
+  return check_launch("pkv_policy_loss_grad");
 }
 
 extern "C" int pkv_scale_grad(void *grad, int64_t n, int32_t dtype, const float *upstream, void *stream) {

@@ -992,13 +992,15 @@ def _policy_forward(logits, tokens, old, ref, adv, mask, kl_coef, clip_low, clip
           _lib.ptr(ref), adv.data_ptr(), adv.stride(0), adv.stride(1) if adv.ndim == 2 else 0, _lib.ptr(mask), batch,
           length, vocab, batch_stride, row_stride, temperature, clip_low, clip_high, kl_coef, reduction,
           out.data_ptr(), logp.data_ptr(), _lib.ptr(grad), ws.data_ptr(), ws_bytes, _status_ptr(status))
-    return out[0], logp, out[1], out[2], grad
+    return out[0], logp, out[1], out[2], grad, ws
 
 
 class _PolicyLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, args):  # (one argument for all constants: apply looks at each)
-        loss, logp, kl, clipped, ctx.d_logits = _policy_forward(logits, *args, True)
+        loss, logp, kl, clipped, ctx.d_logits, ctx.workspace = _policy_forward(logits, *args, True)
+        ctx.save_for_backward(logits)
+        ctx.temperature = args[-3]
         ctx.mark_non_differentiable(logp, kl, clipped)
         ctx.set_materialize_grads(False)  # (no zeros for the outputs without a gradient)
         return loss, logp, kl, clipped
@@ -1008,11 +1010,16 @@ class _PolicyLossFn(torch.autograd.Function):
         _first_order("policy_loss")
         if d_loss is None:
             return None, None
+        (logits,) = ctx.saved_tensors
         grad, ctx.d_logits = ctx.d_logits, None
         if grad is None:
             raise RuntimeError("policy_loss: its gradient was computed with the loss and has been handed out; call "
                                "policy_loss again for another backward pass.")
-        _call(grad.device, "pkv_scale_grad", grad.data_ptr(), grad.numel(), _DTYPES[grad.dtype], d_loss.data_ptr())
+        ws, ctx.workspace = ctx.workspace, None
+        # for an upstream gradient other than 1: read on the device, so nothing waits for it here
+        src, _, _, batch_stride, row_stride = _logit_rows(logits)
+        _call(grad.device, "pkv_policy_loss_grad", src.data_ptr(), _DTYPES[src.dtype], *grad.shape, batch_stride,
+              row_stride, ctx.temperature, ws.data_ptr(), ws.numel(), d_loss.data_ptr(), grad.data_ptr())
         return grad, None
 
 
@@ -1046,9 +1053,12 @@ def policy_loss(
     tokens) or "sum".
 
     Where the logits require grad, the same launch that computes the loss
-    writes their gradient (read once, written once); backward hands it out,
-    scaled by the upstream gradient if that is not 1, so it can run once per
-    call. The other tensors are constants (C ABI pkv_policy_loss).
+    writes their gradient (read once, written once), and backward hands it out,
+    so it can run once per call. Where the upstream gradient is not 1 (a scaled
+    loss, a mean over accumulated batches), backward computes it again from the
+    logits, which are kept until then, with the upstream in fp32: one rounding
+    to the logits' dtype either way. The other tensors are constants (C ABI
+    pkv_policy_loss, pkv_policy_loss_grad).
     """
     _check_logits(logits, tokens, temperature, (3,))
     _dtype_code(logits, "logits")

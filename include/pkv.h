@@ -501,10 +501,18 @@ int pkv_linear_fp8(const void *x, const float *x_scale, const void *w, const flo
  * mask is 0; their logits and tokens are not read. tokens, old_logprobs,
  * ref_logprobs, mask are contiguous; advantages have two strides (0 to
  * broadcast). The workspace is pkv_policy_loss_workspace_size bytes, 16-byte
- * aligned, and may be reused once the call has run.
+ * aligned, and may be reused once the call has run, or, where a gradient for an
+ * upstream is wanted, once pkv_policy_loss_grad has.
+ *
+ * pkv_policy_loss_grad: turns the d_logits that a pkv_policy_loss call wrote into
+ * *upstream (fp32, on the device) times that gradient, computed again from the
+ * logits (unchanged since, the same arguments) and that call's workspace, so each
+ * element is rounded once. Nothing is read or written where *upstream is 1, and
+ * rows with a zero gradient stay as they are.
  *
  * pkv_scale_grad: grad[i] *= *upstream for i < n; returns without touching grad
- * where *upstream is 1.
+ * where *upstream is 1. The product of a stored 16-bit gradient is rounded a
+ * second time, and what was below the type's smallest step stays zero.
  */
 enum {
     PKV_REDUCE_TOKEN = 0,
@@ -532,6 +540,11 @@ int pkv_policy_loss(const void *logits, int32_t dtype, const int64_t *tokens, co
                     float clip_low, float clip_high, float kl_coef, int32_t reduction, float *out,
                     float *logprobs, void *d_logits, void *workspace, size_t workspace_bytes,
                     int32_t *status, void *stream);
+
+int pkv_policy_loss_grad(const void *logits, int32_t dtype, int32_t batch, int32_t length, int32_t vocab,
+                         int64_t batch_stride, int64_t row_stride, float temperature,
+                         const void *workspace, size_t workspace_bytes, const float *upstream,
+                         void *d_logits, void *stream);
 
 int pkv_scale_grad(void *grad, int64_t n, int32_t dtype, const float *upstream, void *stream);
 
