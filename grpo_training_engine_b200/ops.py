@@ -992,7 +992,9 @@ def _policy_forward(logits, tokens, old, ref, adv, mask, kl_coef, clip_low, clip
           _lib.ptr(ref), adv.data_ptr(), adv.stride(0), adv.stride(1) if adv.ndim == 2 else 0, _lib.ptr(mask), batch,
           length, vocab, batch_stride, row_stride, temperature, clip_low, clip_high, kl_coef, reduction,
           out.data_ptr(), logp.data_ptr(), _lib.ptr(grad), ws.data_ptr(), ws_bytes, _status_ptr(status))
-    return out[0], logp, out[1], out[2], grad, ws
+    # .data: tensors of their own, not views of one (a Function's output that is a view cannot be changed in place)
+    loss, kl, clipped = (t.data for t in out.unbind())
+    return loss, logp, kl, clipped, grad, ws
 
 
 class _PolicyLossFn(torch.autograd.Function):
