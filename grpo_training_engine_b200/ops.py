@@ -993,15 +993,15 @@ def _policy_forward(logits, tokens, old, ref, adv, mask, kl_coef, clip_low, clip
           length, vocab, batch_stride, row_stride, temperature, clip_low, clip_high, kl_coef, reduction,
           out.data_ptr(), logp.data_ptr(), _lib.ptr(grad), ws.data_ptr(), ws_bytes, _status_ptr(status))
     # .data: tensors of their own, not views of one (a Function's output that is a view cannot be changed in place)
-    loss, kl, clipped = (t.data for t in out.unbind())
-    return loss, logp, kl, clipped, grad, ws
+    loss, kl, clipped = out.unbind()
+    return loss.data, logp, kl.data, clipped.data, src, grad, ws, (batch, length, vocab, batch_stride, row_stride)
 
 
 class _PolicyLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, args):  # (one argument for all constants: apply looks at each)
-        loss, logp, kl, clipped, ctx.d_logits, ctx.workspace = _policy_forward(logits, *args, True)
-        ctx.save_for_backward(logits)
+        loss, logp, kl, clipped, src, ctx.d_logits, ctx.workspace, ctx.layout = _policy_forward(logits, *args, True)
+        ctx.save_for_backward(src)
         ctx.temperature = args[-3]
         ctx.mark_non_differentiable(logp, kl, clipped)
         ctx.set_materialize_grads(False)  # (no zeros for the outputs without a gradient)
@@ -1012,16 +1012,15 @@ class _PolicyLossFn(torch.autograd.Function):
         _first_order("policy_loss")
         if d_loss is None:
             return None, None
-        (logits,) = ctx.saved_tensors
+        (src,) = ctx.saved_tensors
         grad, ctx.d_logits = ctx.d_logits, None
         if grad is None:
             raise RuntimeError("policy_loss: its gradient was computed with the loss and has been handed out; call "
                                "policy_loss again for another backward pass.")
         ws, ctx.workspace = ctx.workspace, None
         # for an upstream gradient other than 1: read on the device, so nothing waits for it here
-        src, _, _, batch_stride, row_stride = _logit_rows(logits)
-        _call(grad.device, "pkv_policy_loss_grad", src.data_ptr(), _DTYPES[src.dtype], *grad.shape, batch_stride,
-              row_stride, ctx.temperature, ws.data_ptr(), ws.numel(), d_loss.data_ptr(), grad.data_ptr())
+        _call(grad.device, "pkv_policy_loss_grad", src.data_ptr(), _DTYPES[src.dtype], *ctx.layout, ctx.temperature,
+              ws.data_ptr(), ws.numel(), d_loss.data_ptr(), grad.data_ptr())
         return grad, None
 
 
