@@ -22,6 +22,7 @@ from dataclasses import dataclass
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -881,6 +882,8 @@ def _check_logits(logits: torch.Tensor, tokens: torch.Tensor, temperature: float
                          f"{tuple(tokens.shape)}.")
     if not temperature > 0.0:
         raise ValueError("temperature must be > 0.")
+    if forward_ad.unpack_dual(logits).tangent is not None:
+        raise RuntimeError("logits carry a forward-mode tangent; only backward derivatives are implemented.")
 
 
 def _tokens64(tokens: torch.Tensor) -> torch.Tensor:
