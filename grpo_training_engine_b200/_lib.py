@@ -39,6 +39,7 @@ DEV_TOKEN_OUT_OF_RANGE = 8  # PKV_DEV_TOKEN_OUT_OF_RANGE
 REDUCE_TOKEN = 0  # PKV_REDUCE_TOKEN
 REDUCE_SEQUENCE = 1  # PKV_REDUCE_SEQUENCE
 REDUCE_SUM = 2  # PKV_REDUCE_SUM
+POLICY_TEST_WAIT_TIMEOUT = 1 << 30  # PKV_POLICY_TEST_WAIT_TIMEOUT (tests of the bounded waits only)
 
 DECODE_FORCE_GENERIC = 1
 DECODE_EXACT_P = 2

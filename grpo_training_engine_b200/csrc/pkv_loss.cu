@@ -485,6 +485,8 @@ struct PolicyArgs {
   int32_t batch, length, vocab, reduction;
   int32_t ctas, hold;  // CTAs of a row (loss alone); vectors of a row kept in shared memory (gradient)
   float inv_t, c, clip_low, clip_high, kl_coef;
+  uint32_t max_polls;  // limit of each wait of the ring
+  int32_t withhold;    // PKV_POLICY_TEST_WAIT_TIMEOUT: the first CTA leaves out its second row's last chunk
 };
 
 constexpr int kPrepThreads = 1024;
@@ -805,13 +807,21 @@ policy_row_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
 // 481 us. (Before: a block per row with two reads 1114 us; a cluster of 8 per row
 // that holds it, 490; rows summed before the last one is written, 500; chunks
 // of half the size 560.)
+//
+// Every wait is bounded. Where one runs out, its thread waits for nothing more,
+// the consumers take no further row after the next join, the producer waits
+// (bounded) for its copies in flight, and the status gets PKV_DEV_WAIT_TIMEOUT. For
+// a caller without a status, the loss is NaN, and so are the log-probability and the
+// first element of the gradient of each row that is left.
 template <int NT, int K>
 struct GradShared {
   uint64_t full[K], empty[K];  // a chunk has landed, has been used by every warp
-  uint64_t info;                           // token inputs are there
+  uint64_t info;                // token inputs are there
   TokenIn token[2];
   float2 part[NT / 32];
   RowResult result;
+  volatile int dead;  // a wait ran out
+  int stop;           // ... as every consumer sees it after the row's join
 };
 
 template <typename T, int NT, int K, int PerSm>
@@ -829,6 +839,7 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
       mbar_init(&sh.empty[k], NT / 32);
     }
     mbar_init(&sh.info, 1);
+    sh.dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -836,18 +847,20 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
   auto chunk = [](int held, int k) { return min(held, k * NT * kUnroll); };
   bool ok = true;
   Sums sums;
+  int it = 0, k = 0;  // this CTA's row; the producer's chunk of it, 0 once all have been issued
 
   if (warp == NT / 32) {
     // producer
     if (lane == 0) {
-      int it = 0;
       for (int64_t pos = blockIdx.x; pos < active; pos += gridDim.x, ++it) {
         const int64_t r = a.order[pos];
         const T *x = logits + rows.offset(r);
         const Slice<T> sl(x, a.vocab, 0, 1);
         const int held = min(sl.hi, a.hold);
-        for (int k = 0; k < K; ++k) {
-          if (it > 0) ok = mbar_wait_bounded(&sh.empty[k], (it - 1) & 1) && ok;
+        for (k = 0; k < K; ++k) {
+          if (it > 0) ok = mbar_wait_bounded(&sh.empty[k], (it - 1) & 1, a.max_polls);
+          if (!ok) break;
+          if (a.withhold && blockIdx.x == 0 && it == 1 && k == K - 1) continue;
           if (k == K / 2 && sl.hi > held)  // what is not held, on its way to L2 before the consumers stream it
             asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(sl.vecs() + held),
                          "r"((sl.hi - held) * 16)
@@ -861,6 +874,8 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
                 "l"(sl.vecs() + c0), "r"(bytes), "r"(smem_u32(&sh.full[k]))
                 : "memory");
         }
+        if (!ok) break;
+        k = 0;
         // slot it & 1 was last read for row it - 2, before any chunk of row it - 1 was free
         sh.token[it & 1] = token_in(a, x, r);
         mbar_arrive(&sh.info);
@@ -871,22 +886,24 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
     // this thread's part of chunk k of the it-th row of this CTA
     auto sum_chunk = [&](Soft &st, int held, int k, int it) {
       const int c0 = chunk(held, k), c1 = chunk(held, k + 1);
-      ok = mbar_wait_bounded(&sh.full[k], it & 1) && ok;
-      add_range<T, false, NT, false>(st, hv + c0, c1 - c0, a.c, tid);
+      if (ok) ok = mbar_wait_bounded(&sh.full[k], it & 1, a.max_polls);
+      if (ok)
+        add_range<T, false, NT, false>(st, hv + c0, c1 - c0, a.c, tid);
+      else
+        sh.dead = 1;
     };
     auto sum_rest = [&](Soft &st, const Slice<T> &sl, int held) {
       add_range<T, false, NT, true>(st, sl.vecs() + held, sl.hi - held, a.c, tid);
       const int e = sl.edge(tid);
       if (e >= 0) add<false>(st, Elem<T>::to_f32(sl.x[e]), a.c);
     };
-    int it = 0;
     int64_t pos = blockIdx.x, r = a.order[pos];
     Soft st;
     if (pos < active) {
       const Slice<T> sl(logits + rows.offset(r), a.vocab, 0, 1);
       const int held = min(sl.hi, a.hold);
       sum_rest(st, sl, held);
-      for (int k = 0; k < K; ++k) sum_chunk(st, held, k, 0);
+      for (k = 0; k < K; ++k) sum_chunk(st, held, k, 0);
     }
     for (; pos < active; pos += gridDim.x, ++it) {
       const bool more = pos + gridDim.x < active;
@@ -902,11 +919,17 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
           st.s = sh.part[lane].y;
         }
         warp_join<false>(st, a.c);
-        ok = mbar_wait_bounded(&sh.info, it & 1) && ok;
-        if (lane == 0) sh.result = token_result(a, sh.token[it & 1], st, r, sums);
+        if (ok) ok = mbar_wait_bounded(&sh.info, it & 1, a.max_polls);
+        if (!ok) sh.dead = 1;
+        __syncwarp();
+        if (lane == 0) {
+          sh.stop = sh.dead;
+          if (!sh.stop) sh.result = token_result(a, sh.token[it & 1], st, r, sums);
+        }
         __syncwarp();
       }
       bar_sync<NT>();
+      if (sh.stop) break;
       const Slope g{sh.result.m, a.c, sh.result.k, 0.f, sh.result.slope, sh.result.tok};
       const Slice<T> sl(logits + rows.offset(r), a.vocab, 0, 1), sn(logits + rows.offset(next), a.vocab, 0, 1);
       const int held = min(sl.hi, a.hold), held_n = min(sn.hi, a.hold);
@@ -915,7 +938,7 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
       // what is not held first: it is the longest since it was read, and the chunks' refills are then in flight
       // until the end
       grad_range<T, false, NT>(sl, g, out, sl.vecs() + held, held, sl.hi, tid);
-      for (int k = 0; k < K; ++k) {
+      for (k = 0; k < K; ++k) {
         const int c0 = chunk(held, k), c1 = chunk(held, k + 1);
         grad_range<T, false, NT>(sl, g, out, hv + c0, c0, c1, tid);
         __syncwarp();
@@ -929,10 +952,24 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
       }
       r = next;
     }
+    for (; pos < active; pos += gridDim.x) {  // (only after a wait that ran out)
+      r = a.order[pos];
+      if (tid == 0) {
+        grad[r * (int64_t)a.vocab] = from_f32<T>(NAN);
+        a.logp[r] = NAN;
+        a.slopes[r] = make_float4(NAN, NAN, NAN, __int_as_float(-1));
+      }
+    }
     for (; pos < n; pos += gridDim.x) zero_row<T, NT>(a, grad, a.order[pos], tid);
   }
   if (!ok) flag_status(a.status, PKV_DEV_WAIT_TIMEOUT);
-  __syncthreads();
+  if (__syncthreads_or(!ok)) {
+    sums.loss = sums.kl = sums.clipped = NAN;
+    // copies in flight land before the shared memory goes away: the chunks before k for row it, the others for the last
+    if (tid == NT && it + k > 0)
+      for (int j = 0; j < K; ++j)
+        if (!mbar_wait_bounded(&sh.full[j], (j < k ? it : it - 1) & 1, a.max_polls)) break;
+  }
   finish<NT + 32>(a, sums, blockIdx.x, gridDim.x);
 }
 
@@ -1149,6 +1186,8 @@ extern "C" int pkv_policy_loss(const void *logits, int32_t dtype, const int64_t 
                                int32_t *status, void *stream) {
   if (dtype_size(dtype) == 0) return PKV_ERR_UNSUPPORTED;
   const int64_t rows = (int64_t)batch * length;
+  const bool test_timeout = (reduction & PKV_POLICY_TEST_WAIT_TIMEOUT) != 0;
+  reduction &= ~PKV_POLICY_TEST_WAIT_TIMEOUT;
   if (batch < 0 || length < 0 ||
       bad_logits("pkv_policy_loss", logits, dtype, rows, vocab, std::max(1, length), temperature))
     return PKV_ERR_INVALID_ARG;
@@ -1166,6 +1205,8 @@ extern "C" int pkv_policy_loss(const void *logits, int32_t dtype, const int64_t 
   if (!workspace || workspace_bytes < pkv_policy_loss_workspace_size(batch, length) || !aligned_to(workspace, 16))
     return PKV_ERR_WORKSPACE;
   PolicyArgs a{};
+  a.max_polls = test_timeout ? 4096 : kMaxPolls;
+  a.withhold = test_timeout;
   a.tokens = tokens;
   a.old_logp = old_logprobs;
   a.ref_logp = ref_logprobs;

@@ -502,7 +502,9 @@ int pkv_linear_fp8(const void *x, const float *x_scale, const void *w, const flo
  * ref_logprobs, mask are contiguous; advantages have two strides (0 to
  * broadcast). The workspace is pkv_policy_loss_workspace_size bytes, 16-byte
  * aligned, and may be reused once the call has run, or, where a gradient for an
- * upstream is wanted, once pkv_policy_loss_grad has.
+ * upstream is wanted, once pkv_policy_loss_grad has. A wait inside the gradient's
+ * kernel that runs out sets PKV_DEV_WAIT_TIMEOUT; out, and the log-probabilities
+ * and the first gradient of each row that was left out, are then NaN.
  *
  * pkv_policy_loss_grad: turns the d_logits that a pkv_policy_loss call wrote into
  * *upstream (fp32, on the device) times that gradient, computed again from the
@@ -517,7 +519,10 @@ int pkv_linear_fp8(const void *x, const float *x_scale, const void *w, const flo
 enum {
     PKV_REDUCE_TOKEN = 0,
     PKV_REDUCE_SEQUENCE = 1,
-    PKV_REDUCE_SUM = 2
+    PKV_REDUCE_SUM = 2,
+    PKV_POLICY_TEST_WAIT_TIMEOUT = 1 << 30 /* TEST ONLY, OR'd into reduction (gradient of rows over 64 KB): the
+                                              waits' limits are 4096 polls and the first CTA leaves out the last
+                                              part of its second row, so that they run out */
 };
 
 int pkv_token_logprobs(const void *logits, int32_t dtype, const int64_t *tokens, int64_t rows,
