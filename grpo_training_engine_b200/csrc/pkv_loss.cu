@@ -479,7 +479,7 @@ struct PolicyArgs {
   int32_t *order;          // workspace [batch * length]: tokens with a weight first
   int32_t *before;         // workspace [batch + 1]: such tokens before each sequence
   int32_t *counts;         // workspace: [0] tokens with a weight, [1] blocks done
-  float4 *slopes;          // workspace [batch * length], or nullptr: what policy_grad_scaled_kernel takes of a row
+  float4 *slopes;          // workspace [batch * length]: what policy_grad_scaled_kernel takes of a row
   int32_t *status;
   int64_t adv_b, adv_t;
   int32_t batch, length, vocab, reduction;
@@ -608,8 +608,14 @@ __device__ __forceinline__ RowResult token_result(const PolicyArgs &a, const Tok
                   : a.reduction == PKV_REDUCE_SEQUENCE ? 1.f / ((float)t.len * (float)a.batch)
                                                        : 1.f / (float)t.len;
   slope *= w * a.inv_t;
-  const RowResult res{st.m, -slope / st.s, slope, t.tok};
-  if (a.slopes != nullptr) a.slopes[r] = make_float4(res.m, res.k, res.slope, __int_as_float(t.in ? (int)t.tok : -1));
+  return RowResult{st.m, -slope / st.s, slope, t.tok};
+}
+
+// ... and in a gradient's kernel, kept for policy_grad_scaled_kernel.
+__device__ __forceinline__ RowResult kept_result(const PolicyArgs &a, const TokenIn &t, const Soft &st, int64_t r,
+                                                 Sums &sums) {
+  const RowResult res = token_result(a, t, st, r, sums);
+  a.slopes[r] = make_float4(res.m, res.k, res.slope, __int_as_float(t.in ? (int)t.tok : -1));
   return res;
 }
 
@@ -762,7 +768,7 @@ policy_row_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
         warp_join<false>(st, a.c);
       }
     }
-    if (tid == 0) result[group] = token_result(a, t, st, r, sums);
+    if (tid == 0) result[group] = kept_result(a, t, st, r, sums);
     sync();
     const RowResult res = result[group];
     const Slope g{res.m, a.c, res.k, 0.f, res.slope, res.tok};
@@ -924,7 +930,7 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
         __syncwarp();
         if (lane == 0) {
           sh.stop = sh.dead;
-          if (!sh.stop) sh.result = token_result(a, sh.token[it & 1], st, r, sums);
+          if (!sh.stop) sh.result = kept_result(a, sh.token[it & 1], st, r, sums);
         }
         __syncwarp();
       }
@@ -1218,7 +1224,7 @@ extern "C" int pkv_policy_loss(const void *logits, int32_t dtype, const int64_t 
   const PolicyWorkspace w = policy_workspace(batch, length);
   a.partial = reinterpret_cast<double *>(ws);
   a.counts = reinterpret_cast<int32_t *>(ws + w.counts);
-  a.slopes = d_logits ? reinterpret_cast<float4 *>(ws + w.slopes) : nullptr;
+  a.slopes = reinterpret_cast<float4 *>(ws + w.slopes);
   a.order = reinterpret_cast<int32_t *>(ws + w.order);
   a.before = reinterpret_cast<int32_t *>(ws + w.before);
   a.status = status;
