@@ -265,17 +265,15 @@ extern "C" int pkv_add_rmsnorm_fp8(const void *x, const void *residual, const vo
     return PKV_ERR_INVALID_ARG;
   }
   if (rows == 0) return PKV_OK;
-  const void *ptrs[] = {x, residual, weight, sum_out};
-  for (const void *p : ptrs)
-    if (!aligned_to(p, es)) return PKV_ERR_ALIGNMENT;
+  if (!all_aligned(es, {x, residual, weight, sum_out}) || !aligned_to(scales, 4)) return PKV_ERR_ALIGNMENT;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const NormArgs a{x, residual, weight, sum_out, (uint8_t *)q_out, scales, x_stride, residual_stride, sum_stride,
                    q_stride, scale_stride, hidden, eps};
   // 16-byte vectors where every row begins on one; q's rows take the vectors' 8-bit images
   const int n = 16 / es;
   const int64_t strides[] = {x_stride, residual ? residual_stride : 0, sum_out ? sum_stride : 0};
-  bool vec = hidden % n == 0 && hidden / n <= 2 * 1024 && aligned_to(q_out, n) && q_stride % n == 0;
-  for (const void *p : ptrs) vec = vec && aligned_to(p, 16);
+  bool vec = hidden % n == 0 && hidden / n <= 2 * 1024 && aligned_to(q_out, n) && q_stride % n == 0 &&
+             all_aligned(16, {x, residual, weight, sum_out});
   for (int64_t v : strides) vec = vec && v % n == 0;
   if (!vec) {
     PKV_BY_DTYPE(dtype, (norm_fp8_any_kernel<T><<<rows, kAnyThreads, 0, st>>>(a)))
@@ -309,7 +307,7 @@ extern "C" int pkv_quantize_fp8(const void *x, void *q_out, float *scales, int64
     return PKV_ERR_INVALID_ARG;
   }
   if (rows == 0) return PKV_OK;
-  if (!aligned_to(x, es)) return PKV_ERR_ALIGNMENT;
+  if (!aligned_to(x, es) || !aligned_to(scales, 4)) return PKV_ERR_ALIGNMENT;
   const int64_t blocks = (rows + block_rows - 1) / block_rows * groups;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   PKV_BY_DTYPE(dtype, {

@@ -666,9 +666,9 @@ extern "C" int pkv_linear_fp8(const void *x, const float *x_scale, const void *w
     return PKV_ERR_INVALID_ARG;
   }
   if (!aligned_to(x, 16) || !aligned_to(w, 16) || x_stride < k || w_stride < k || x_stride % 16 != 0 ||
-      w_stride % 16 != 0 || !aligned_to(x_scale, 4) || !aligned_to(w_scale, 4) || !aligned_to(out, 2) ||
-      !aligned_to(bias, 2)) {
-    set_error_detail("pkv_linear_fp8: x and W need 16-byte aligned bases and row strides (x %lld, W %lld)",
+      w_stride % 16 != 0 || !all_aligned(4, {x_scale, w_scale, status}) || !all_aligned(2, {out, bias})) {
+    set_error_detail("pkv_linear_fp8: x and W need 16-byte aligned bases and row strides (x %lld, W %lld), the "
+                     "others their elements' alignment",
                      (long long)x_stride, (long long)w_stride);
     return PKV_ERR_ALIGNMENT;
   }

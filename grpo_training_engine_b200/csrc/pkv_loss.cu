@@ -1123,8 +1123,8 @@ extern "C" int pkv_token_logprobs(const void *logits, int32_t dtype, const int64
   if (dtype_size(dtype) == 0) return PKV_ERR_UNSUPPORTED;
   if (bad_logits("pkv_token_logprobs", logits, dtype, rows, vocab, inner, temperature)) return PKV_ERR_INVALID_ARG;
   if (rows == 0) return PKV_OK;
-  if (!tokens || !logprobs) {
-    set_error_detail("pkv_token_logprobs: NULL pointer");
+  if (!tokens || !logprobs || !all_aligned(8, {tokens, stats}) || !all_aligned(4, {logprobs, entropy, status})) {
+    set_error_detail("pkv_token_logprobs: NULL or misaligned pointer");
     return PKV_ERR_INVALID_ARG;
   }
   const Rows rw{outer_stride, row_stride, inner};
@@ -1152,7 +1152,8 @@ extern "C" int pkv_token_logprobs_grad(const void *logits, int32_t dtype, const 
   if (bad_logits("pkv_token_logprobs_grad", logits, dtype, rows, vocab, inner, temperature))
     return PKV_ERR_INVALID_ARG;
   if (rows == 0) return PKV_OK;
-  if (!tokens || !stats || !d_logits || (d_entropy && !entropy) || !aligned_to(d_logits, dtype_size(dtype))) {
+  if (!tokens || !stats || !d_logits || (d_entropy && !entropy) || !aligned_to(d_logits, dtype_size(dtype)) ||
+      !all_aligned(8, {tokens, stats}) || !all_aligned(4, {entropy, d_logprobs, d_entropy})) {
     set_error_detail("pkv_token_logprobs_grad: NULL or misaligned pointer");
     return PKV_ERR_INVALID_ARG;
   }
@@ -1203,9 +1204,10 @@ extern "C" int pkv_policy_loss(const void *logits, int32_t dtype, const int64_t 
     return out ? check_launch("pkv_policy_loss") : PKV_ERR_INVALID_ARG;
   }
   if (!tokens || !old_logprobs || !advantages || !out || !logprobs || !aligned_to(d_logits, dtype_size(dtype)) ||
+      !aligned_to(tokens, 8) || !all_aligned(4, {old_logprobs, ref_logprobs, advantages, out, logprobs, status}) ||
       !(clip_low >= 0.f) || !(clip_high >= 0.f) || reduction < PKV_REDUCE_TOKEN || reduction > PKV_REDUCE_SUM) {
-    set_error_detail("pkv_policy_loss: NULL pointer, clip range %g / %g or reduction %d", (double)clip_low,
-                     (double)clip_high, reduction);
+    set_error_detail("pkv_policy_loss: NULL or misaligned pointer, clip range %g / %g or reduction %d",
+                     (double)clip_low, (double)clip_high, reduction);
     return PKV_ERR_INVALID_ARG;
   }
   if (!workspace || workspace_bytes < pkv_policy_loss_workspace_size(batch, length) || !aligned_to(workspace, 16))
@@ -1294,8 +1296,8 @@ extern "C" int pkv_policy_loss_grad(const void *logits, int32_t dtype, int32_t b
 
 extern "C" int pkv_scale_grad(void *grad, int64_t n, int32_t dtype, const float *upstream, void *stream) {
   if (dtype_size(dtype) == 0) return PKV_ERR_UNSUPPORTED;
-  if (n < 0 || (n > 0 && (!grad || !upstream))) {
-    set_error_detail("pkv_scale_grad: n %lld or NULL pointer", (long long)n);
+  if (n < 0 || (n > 0 && (!grad || !upstream)) || !aligned_to(grad, dtype_size(dtype)) || !aligned_to(upstream, 4)) {
+    set_error_detail("pkv_scale_grad: n %lld, NULL or misaligned pointer", (long long)n);
     return PKV_ERR_INVALID_ARG;
   }
   if (n == 0) return PKV_OK;

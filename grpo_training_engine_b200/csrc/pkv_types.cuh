@@ -2,6 +2,8 @@
 // dispatch over element types of the scoring and update kernels.
 #pragma once
 
+#include <initializer_list>
+
 #include "pkv_common.cuh"
 
 // Runs the statements with T the element type of `dtype` (a checked code).
@@ -13,6 +15,13 @@
   }
 
 namespace pkv {
+
+// Whether every pointer (NULL ones too) is a multiple of `size`: a misaligned one would fault in the kernel.
+inline bool all_aligned(size_t size, std::initializer_list<const void *> ptrs) {
+  for (const void *p : ptrs)
+    if (!aligned_to(p, size)) return false;
+  return true;
+}
 
 template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
