@@ -985,8 +985,9 @@ policy_grad_kernel(const T *logits, Rows rows, T *grad, PolicyArgs a) {
 // the type's smallest step would have been lost before a loss scale could lift it.
 // Nothing to do where u is 1, or in a row whose gradient is zero (no weight, or
 // clipped): policy_loss wrote that. NT threads per row, or per share of one (ctas of
-// them, no larger than 64 KB); a persistent grid, since a launch for u = 1 should
-// cost no more than a launch.
+// them, of 64 KB and less); a persistent grid, since a launch for u = 1 should cost
+// no more than a launch (1.6 us). Bound by HBM: 2752 of 4096 rows of 151,936 bf16
+// take 292 us, 5.7 TB/s of what is read and written.
 template <typename T, int NT>
 __global__ void __launch_bounds__(kThreads, 4)
 policy_grad_scaled_kernel(const T *logits, Rows rows, T *grad, const float4 *slopes, const int32_t *order,

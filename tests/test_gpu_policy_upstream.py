@@ -10,7 +10,7 @@ from test_gpu_policy import DTYPES, _batch, _check_grad, _policy_formula
 pytestmark = pytest.mark.gpu
 
 if torch.cuda.is_available():
-    from grpo_training_engine_b200 import ops
+    from grpo_training_engine_b200 import _lib, ops
 
 
 @pytest.mark.parametrize("upstream", [65536.0, 3.0, 1.0 / 3.0, -0.7, 1.0, 0.0])
@@ -67,3 +67,15 @@ def test_empty_batch_under_an_upstream():
                           torch.empty(0, device="cuda"))
     (got.loss * 3).backward()
     assert leaf.grad.shape == (0, 4, 10)
+
+
+@pytest.mark.parametrize("n", [1, 1000, 1 << 20])
+def test_scale_grad_in_place(n):
+    """The C entry point that multiplies a stored fp32 gradient; an upstream of 1 leaves it as it is."""
+    grad = torch.randn(n, device="cuda")
+    want = grad * 3
+    for u, expect in ((1.0, grad.clone()), (3.0, want)):
+        up = torch.tensor(u, device="cuda")
+        rc = _lib.load().pkv_scale_grad(grad.data_ptr(), n, _lib.DTYPE_F32, up.data_ptr(),
+                                        torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(grad, expect)
